@@ -174,6 +174,105 @@ int tt_ffn_residual_layernorm(const void* a, const void* w1, const float* b1, co
  * (host).  Returns TT_OK, or TT_ERR_UNSUPPORTED for shapes outside it. */
 int tt_route_describe(int d_model, int heads, int seq, int ffn, char* buf, int buflen);
 
+/* ---- paged K/V cache -------------------------------------------------------
+ *
+ * For answering token by token.  The reference has no cache (every call of
+ * mixed_precision/transformer.py:480-699 recomputes the whole sequence).
+ *
+ * A pool holds n_pages pages of every layer.  A page is [kv_heads, page,
+ * head_dim] 16-bit values of K, contiguous, and the same of V; layers and pages
+ * may be any stride apart.  tables[slot][i] is the page of a sequence's tokens
+ * i*page .. (i+1)*page - 1 (-1: none), lens[slot] its length, refs[p] the number
+ * of table entries that name page p (0: free).  head_dim 8 is stored 16 wide,
+ * as everywhere in this library.  Batch entry b of a call is slot slots[b], or
+ * slot b when slots is NULL; its new tokens are the rows cu_q[b] .. cu_q[b+1]
+ * - 1 of the call's token tensors.  Bookkeeping runs on the device; no entry
+ * point synchronizes.  Page indices outside the pool and slots outside the
+ * table are skipped, never dereferenced. */
+typedef struct tt_kv_cache {
+  void* k;                 /* first layer's pages; may be NULL in calls that move no values */
+  void* v;
+  int64_t k_layer_stride;  /* elements between layers */
+  int64_t v_layer_stride;
+  int64_t k_page_stride;   /* elements between pages (a multiple of 8) */
+  int64_t v_page_stride;
+  int* tables;
+  int64_t table_stride;    /* entries between table rows */
+  int* lens;
+  int* refs;               /* may be NULL in calls that use no counts */
+  int layers;
+  int n_pages;
+  int kv_heads;
+  int page;                /* tokens per page: 16, 32, 64, 128 or 256 */
+  int head_dim;            /* as stored: 16, 32, 64, 128 or 256 */
+  int n_slots;
+  int table_width;
+} tt_kv_cache;
+
+/* Makes room for the new tokens of a batch of distinct slots: allocates the
+ * lowest free pages (in batch order), sets their counts to 1, enters them in
+ * the tables and adds the new tokens to lens.  All or nothing.  *status
+ * (device): 0 done; > 0 that many pages are missing; -1 a sequence would
+ * outgrow its table row; -2 a slot outside the table or a decreasing cu_q.
+ * batch <= 32768. */
+int tt_cache_reserve(const tt_kv_cache* cache, const int* cu_q, const int* slots, int batch,
+                     int* status, void* stream);
+
+/* Writes K and V of the new tokens (already counted by lens) into one layer's
+ * pages.  k and v are [n_tokens, kv_heads, head_dim] with element strides
+ * {token, head, feature}: dense in the features (16-byte aligned rows), or
+ * dense in the tokens (tt_qkv_projection's vt). */
+int tt_cache_append(const tt_kv_cache* cache, const void* k, const int64_t* k_strides, const void* v,
+                    const int64_t* v_strides, int n_tokens, const int* cu_q, const int* slots,
+                    int batch, void* stream);
+
+/* Releases pages of n slots (all n_slots when slots is NULL): every page, the
+ * length becoming 0 (window 0), or with a window those pages that no later
+ * query of the slot can see. */
+int tt_cache_release(const tt_kv_cache* cache, const int* slots, int n, int window, int sinks,
+                     void* stream);
+
+/* children[i] (empty, distinct) becomes a copy of parents[i]: it shares the
+ * full pages and gets a page of its own for a partial last one, whose used
+ * rows are copied in every layer.  All or nothing.  *status (device): 0 done;
+ * > 0 pages missing; -1 a parent without its last page; -2 a slot outside the
+ * table; -3 a child that is not empty or occurs twice.  scratch: 2n + 1 ints.
+ * n <= 32768 and n_slots <= 524288. */
+int tt_cache_fork(const tt_kv_cache* cache, const int* parents, const int* children, int n,
+                  int* scratch, int* status, void* stream);
+
+/* Moves the live pages to the front of the pool: with n live pages, the k-th
+ * live page of index >= n goes to the k-th free index below n; tables and refs
+ * follow, *live (device) = n.  scratch: 3 n_pages + 2 ints. */
+int tt_cache_compact(const tt_kv_cache* cache, int* scratch, int* live, void* stream);
+
+/* Copies pages src[i] -> dst[i] (device index lists; no page of dst twice or
+ * in src) of every layer. */
+int tt_cache_copy_pages(const tt_kv_cache* cache, const int* src, const int* dst, int n, void* stream);
+
+/* Attention of the new tokens of a batch over one layer's pages.  Query j of
+ * a sequence of T new tokens and length L (lens, new tokens included) stands
+ * at t = L - T + j and sees key u iff 0 <= u <= t and (window == 0 or
+ * t - u < window or u < sinks); every visible key must have a page.
+ * out[row, h*hd:(h+1)*hd] = softmax(scale q k^T) v over the visible keys, zero
+ * for a row that sees none and for a row of no sequence; FP32 statistics and
+ * accumulation, out in the cache's type.  q: [n_tokens, heads, stored
+ * head_dim], element strides token and head, multiples of 8; query head h
+ * reads KV head h / (heads / kv_heads), heads / kv_heads <= 128.  head_dim: 8
+ * (stored 16 wide), 16, 32, 64, 128 or 256.  max_q_len: an upper bound of T
+ * (<= 0: n_tokens).  is_bf16: type of q, the pages and out (0: FP16).
+ * workspace: tt_paged_attention_workspace_bytes. */
+int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_stride,
+                       int64_t q_head_stride, const int* cu_q, const int* slots, int batch,
+                       void* out, int n_tokens, int heads, int head_dim, int is_bf16, float scale,
+                       int window, int sinks, int max_q_len, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Workspace bytes that tt_paged_attention needs on the current device for
+ * these heads, whatever the batch and the lengths. */
+int tt_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int max_q_len,
+                                       size_t* bytes);
+
 /* ---- whole model ----------------------------------------------------------- */
 
 /* Per-layer parameters (device pointers).  Linear weights are FP16 [out, in]

@@ -67,6 +67,30 @@ class ModelDesc(ctypes.Structure):
     ]
 
 
+class KVCache(ctypes.Structure):
+    """struct tt_kv_cache."""
+
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_layer_stride", c_int64),
+        ("v_layer_stride", c_int64),
+        ("k_page_stride", c_int64),
+        ("v_page_stride", c_int64),
+        ("tables", c_void_p),
+        ("table_stride", c_int64),
+        ("lens", c_void_p),
+        ("refs", c_void_p),
+        ("layers", c_int),
+        ("n_pages", c_int),
+        ("kv_heads", c_int),
+        ("page", c_int),
+        ("head_dim", c_int),
+        ("n_slots", c_int),
+        ("table_width", c_int),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "tt_abi_version": (c_int, []),
@@ -104,6 +128,22 @@ SIGNATURES = {
     ),
     "tt_linear_gelu": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "tt_route_describe": (c_int, [c_int, c_int, c_int, c_int, c_char_p, c_int]),
+    "tt_cache_reserve": (c_int, [POINTER(KVCache), c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "tt_cache_append": (
+        c_int,
+        [POINTER(KVCache), c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_int, c_void_p, c_void_p, c_int,
+         c_void_p],
+    ),
+    "tt_cache_release": (c_int, [POINTER(KVCache), c_void_p, c_int, c_int, c_int, c_void_p]),
+    "tt_cache_fork": (c_int, [POINTER(KVCache), c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "tt_cache_compact": (c_int, [POINTER(KVCache), c_void_p, c_void_p, c_void_p]),
+    "tt_cache_copy_pages": (c_int, [POINTER(KVCache), c_void_p, c_void_p, c_int, c_void_p]),
+    "tt_paged_attention": (
+        c_int,
+        [POINTER(KVCache), c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int,
+         c_float, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p],
+    ),
+    "tt_paged_attention_workspace_bytes": (c_int, [c_int, c_int, c_int, c_int, POINTER(c_size_t)]),
     "tt_model_create": (c_int, [POINTER(ModelDesc), POINTER(c_void_p)]),
     "tt_model_destroy": (None, [c_void_p]),
     "tt_workspace_alloc": (c_int, [c_size_t, POINTER(c_void_p)]),

@@ -1836,3 +1836,5 @@ int tt_model_profile_collect(tt_model* m, float* ms, int* counts, int n) {
 }
 
 }  // extern "C"
+
+#include "tt_cache_api.cuh"

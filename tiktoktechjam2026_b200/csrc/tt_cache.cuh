@@ -1,0 +1,445 @@
+// Paged K/V cache: page bookkeeping (reserve, fork, release, compact) and the
+// kernels that move K and V (append, page copies).
+//
+// A pool holds n_pages pages per layer, a page being [kv_heads, page, HD]
+// 16-bit values of K and the same of V.  tables[slot][i] is the page of the
+// tokens i*page .. (i+1)*page - 1 of a sequence (-1: none), lens[slot] its
+// length, refs[p] the number of table entries that name page p (0: free).
+// All bookkeeping runs on the device, so a decode loop needs no host copy of
+// it; every choice of a page is the lowest free index, so results do not
+// depend on timing.
+#pragma once
+
+#include "tt_ptx.cuh"
+
+namespace tt {
+
+struct CacheParams {
+  uint8_t* k;  // pool of the first layer; a page of one layer is page_bytes contiguous bytes
+  uint8_t* v;
+  long long k_layer, v_layer;  // bytes between layers
+  long long k_stride, v_stride;  // bytes between pages
+  int* tables;
+  long long table_stride;
+  int* lens;
+  int* refs;
+  int layers, n_pages, kv_heads, page_shift, row_bytes;  // row_bytes: HD * 2
+  int n_slots, table_width;
+};
+
+constexpr int kCacheThreads = 1024;
+constexpr int kCacheMaxBatch = 32768;   // sequences of one reserve or fork call (their page counts sit in shared memory)
+constexpr int kCacheMaxSlots = 1 << 19;  // fork marks its children in a shared bitmap
+
+// Block-wide exclusive sum of one int per thread (1024 threads); *total is the sum.
+__device__ __forceinline__ int block_scan(int v, int* total) {
+  __shared__ int warp_sum[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(~0u, inc, o);
+    if (lane >= o) inc += x;
+  }
+  __syncthreads();  // the previous call's sums have been read
+  if (lane == 31) warp_sum[warp] = inc;
+  __syncthreads();
+  int w = warp_sum[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(~0u, w, o);
+    if (lane >= o) w += x;
+  }
+  *total = __shfl_sync(~0u, w, 31);
+  const int before = warp ? __shfl_sync(~0u, w, warp - 1) : 0;
+  return before + inc - v;
+}
+
+constexpr int kScanPer = 8;  // reference counts per thread and step of a scan over the pool
+
+// Number of free pages, counted from page 0 until at least `want` are found.
+__device__ __forceinline__ int count_free(const int* refs, int n_pages, int want) {
+  int found = 0;
+  for (int p0 = 0; p0 < n_pages && found < want; p0 += kCacheThreads * kScanPer) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kScanPer; ++i) {
+      const int p = p0 + i * kCacheThreads + threadIdx.x;
+      if (p < n_pages && refs[p] == 0) ++c;
+    }
+    int total;
+    block_scan(c, &total);
+    found += total;
+  }
+  return found;
+}
+
+// Calls take(k, page) for the first `want` free pages, k = 0, 1, ... in order
+// of the page index, and sets their count to 1.
+template <typename F>
+__device__ __forceinline__ void take_free(int* refs, int n_pages, int want, F take) {
+  int found = 0;
+  for (int p0 = 0; p0 < n_pages && found < want; p0 += kCacheThreads * kScanPer) {
+    const int at = p0 + threadIdx.x * kScanPer;  // consecutive pages per thread: the order of the index
+    unsigned free_bits = 0;
+#pragma unroll
+    for (int i = 0; i < kScanPer; ++i)
+      if (at + i < n_pages && refs[at + i] == 0) free_bits |= 1u << i;
+    int total;
+    int k = found + block_scan(__popc(free_bits), &total);
+    for (; free_bits && k < want; free_bits &= free_bits - 1, ++k) {
+      const int p = at + __ffs(free_bits) - 1;
+      refs[p] = 1;
+      take(k, p);
+    }
+    found += total;
+  }
+}
+
+// Index of the last entry of first[0 .. n - 1] (non-decreasing) that is <= k.
+__device__ __forceinline__ int last_at_most(const int* first, int n, int k) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= k)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// Reserve pages for the new tokens of a batch: sequence b grows by T_b =
+// cu_q[b+1] - cu_q[b], from ceil(L/page) to ceil((L+T)/page) pages.  All or
+// nothing.  One block: the scan over the counts is the whole cost.
+__global__ void __launch_bounds__(kCacheThreads)
+    cache_reserve_kernel(const CacheParams c, const int* cu_q, const int* slots, int batch, int* status) {
+  extern __shared__ int first[];  // [batch]: new pages of the sequences before b
+  const int page = 1 << c.page_shift;
+  int need = 0, bad = 0;
+  for (int b0 = 0; b0 < batch; b0 += kCacheThreads) {
+    const int b = b0 + threadIdx.x;
+    int n = 0;
+    if (b < batch) {
+      const int slot = slots ? slots[b] : b, t = cu_q[b + 1] - cu_q[b];
+      if (slot < 0 || slot >= c.n_slots || t < 0) {
+        bad |= 2;
+      } else {
+        const long long len = c.lens[slot], grown = len + t;
+        if (len < 0 || (grown + page - 1) >> c.page_shift > c.table_width)
+          bad |= 1;
+        else
+          n = static_cast<int>(((grown + page - 1) >> c.page_shift) - ((len + page - 1) >> c.page_shift));
+      }
+    }
+    int total;
+    const int before = block_scan(n, &total);
+    if (b < batch) first[b] = need + before;
+    need += total;
+  }
+  bad = __syncthreads_or(bad & 2) ? -2 : (__syncthreads_or(bad & 1) ? -1 : 0);
+  if (bad) {
+    if (threadIdx.x == 0) *status = bad;
+    return;
+  }
+  const int found = count_free(c.refs, c.n_pages, need);
+  if (threadIdx.x == 0) *status = max(need - found, 0);
+  if (found < need) return;
+  __syncthreads();
+  take_free(c.refs, c.n_pages, need, [&](int k, int p) {
+    const int b = last_at_most(first, batch, k);
+    const int slot = slots ? slots[b] : b;
+    const int old = (c.lens[slot] + page - 1) >> c.page_shift;
+    c.tables[slot * c.table_stride + old + k - first[b]] = p;
+  });
+  __syncthreads();  // every length has been read
+  for (int b = threadIdx.x; b < batch; b += kCacheThreads) c.lens[slots ? slots[b] : b] += cu_q[b + 1] - cu_q[b];
+}
+
+// Writes the new tokens' K and V into their pages: token j of sequence b goes
+// to position L - T + j (lens counts it already).  One block per 64 tokens and
+// KV head; a source is dense in its features (16-byte pieces) or in its tokens
+// (the transposed V of the QKV projection, turned in shared memory).
+struct AppendSrc {
+  const uint16_t* p;
+  long long token, head, feature;  // element strides; feature == 1 or token == 1
+};
+constexpr int kAppendTokens = 64;
+constexpr int kAppendThreads = 256;
+
+__device__ __forceinline__ void append_one(const CacheParams& c, const AppendSrc& s, uint8_t* pool, long long page_stride,
+                                           int t0, int n, int h, int hd, const int* dst_page, const int* dst_row,
+                                           uint16_t* tile) {
+  const int pieces = hd / 8;
+  const uint16_t* src = s.p + h * s.head + t0 * s.token;
+  const long long head_off = (static_cast<long long>(h) << c.page_shift) * c.row_bytes;
+  if (s.feature == 1) {
+    for (int x = threadIdx.x; x < n * pieces; x += kAppendThreads) {
+      const int t = x / pieces, d = x % pieces;
+      if (dst_page[t] < 0) continue;
+      const uint4 v = *reinterpret_cast<const uint4*>(src + t * s.token + d * 8);
+      *reinterpret_cast<uint4*>(pool + dst_page[t] * page_stride + head_off + dst_row[t] * c.row_bytes + d * 16) = v;
+    }
+    return;
+  }
+  constexpr int TS = kAppendTokens + 2;  // an odd number of 32-bit words: a column's entries fall into different banks
+  for (int x = threadIdx.x; x < hd * kAppendTokens; x += kAppendThreads) {
+    const int d = x / kAppendTokens, t = x % kAppendTokens;
+    if (t < n) tile[d * TS + t] = src[d * s.feature + t];
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < n * pieces; x += kAppendThreads) {
+    const int t = x / pieces, d = x % pieces;
+    if (dst_page[t] < 0) continue;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = tile[(d * 8 + 2 * i) * TS + t] | (static_cast<uint32_t>(tile[(d * 8 + 2 * i + 1) * TS + t]) << 16);
+    *reinterpret_cast<uint4*>(pool + dst_page[t] * page_stride + head_off + dst_row[t] * c.row_bytes + d * 16) =
+        make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(kAppendThreads)
+    cache_append_kernel(const CacheParams c, const AppendSrc k, const AppendSrc v, const int* cu_q, const int* slots,
+                        int batch, int n_tokens) {
+  extern __shared__ uint16_t tile[];
+  __shared__ int dst_page[kAppendTokens], dst_row[kAppendTokens];
+  const int t0 = blockIdx.x * kAppendTokens, h = blockIdx.y, hd = c.row_bytes / 2;
+  const int n = min(kAppendTokens, n_tokens - t0);
+  // b0: the last sequence that begins at or before token t0.
+  int b0 = -1;
+  for (int b = 0; b < batch; b += kAppendThreads)
+    b0 += __syncthreads_count(b + static_cast<int>(threadIdx.x) < batch && cu_q[b + threadIdx.x] <= t0);
+  if (static_cast<int>(threadIdx.x) < n) {
+    const int tok = t0 + threadIdx.x;
+    int page = -1, at = 0;
+    int b = b0 + static_cast<int>(threadIdx.x);  // right where every sequence has one new token
+    if (!(b0 >= 0 && b < batch && cu_q[b] <= tok && tok < cu_q[b + 1]))
+      b = batch > 0 && cu_q[0] <= tok ? last_at_most(cu_q, batch, tok) : -1;
+    if (b >= 0 && tok < cu_q[b + 1]) {
+      const int slot = slots ? slots[b] : b;
+      if (slot >= 0 && slot < c.n_slots) {
+        const int pos = c.lens[slot] - cu_q[b + 1] + tok;
+        const int i = pos >> c.page_shift;
+        if (pos >= 0 && i < c.table_width) page = c.tables[slot * c.table_stride + i];
+        if (page >= c.n_pages) page = -1;
+        at = pos & ((1 << c.page_shift) - 1);
+      }
+    }
+    dst_page[threadIdx.x] = page;
+    dst_row[threadIdx.x] = at;
+  }
+  __syncthreads();
+  append_one(c, k, c.k, c.k_stride, t0, n, h, hd, dst_page, dst_row, tile);
+  append_one(c, v, c.v, c.v_stride, t0, n, h, hd, dst_page, dst_row, tile);
+}
+
+// Releases the pages of `n` slots: all of them (window 0; the length becomes
+// 0), or those that no later query of the slot can see under the window, i.e.
+// whose tokens are all past the first `sinks` and more than window - 1 behind
+// position lens.  The exchange hands each entry's page to one thread, so a
+// slot listed twice is released once.
+__global__ void __launch_bounds__(256)
+    cache_release_kernel(const CacheParams c, const int* slots, int n, int window, int sinks) {
+  const int slot = slots ? slots[blockIdx.x] : static_cast<int>(blockIdx.x);
+  if (slot < 0 || slot >= c.n_slots) return;
+  int* row = c.tables + slot * c.table_stride;
+  int lo = 0, hi = c.table_width;
+  if (window > 0) {
+    const int page = 1 << c.page_shift;
+    lo = static_cast<int>((static_cast<long long>(sinks) + page - 1) >> c.page_shift);
+    const long long behind = static_cast<long long>(c.lens[slot]) - window + 1;
+    hi = behind > 0 ? static_cast<int>(min(behind >> c.page_shift, static_cast<long long>(c.table_width))) : 0;
+  }
+  for (int i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+    const int p = row[i] < 0 ? -1 : atomicExch(row + i, -1);
+    if (p >= 0 && p < c.n_pages) atomicSub(c.refs + p, 1);
+  }
+  if (window == 0 && threadIdx.x == 0) c.lens[slot] = 0;
+}
+
+// Moves `bytes` (a multiple of 16) with the whole block, eight 16-byte pieces per thread in flight.
+__device__ __forceinline__ void copy_block(uint8_t* dst, const uint8_t* src, int bytes) {
+  constexpr int U = 8;
+  const int n = bytes / 16, step = blockDim.x * U;
+  const uint4* s = reinterpret_cast<const uint4*>(src);
+  uint4* d = reinterpret_cast<uint4*>(dst);
+  for (int i = threadIdx.x; i < n; i += step) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * static_cast<int>(blockDim.x) < n) v[u] = __ldcs(s + i + u * blockDim.x);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * static_cast<int>(blockDim.x) < n) __stcs(d + i + u * blockDim.x, v[u]);
+  }
+}
+
+// Bookkeeping of fork: checks every pair, then gives each child with a partial
+// last page the next free page.  scratch: [0] go, then per pair its length and
+// its new page (-1: none).
+__global__ void __launch_bounds__(kCacheThreads)
+    cache_fork_plan_kernel(const CacheParams c, const int* parents, const int* children, int n, int* scratch,
+                           int* status) {
+  extern __shared__ int shared[];
+  int* first = shared;                                         // [n]: new pages of the pairs before i
+  unsigned* seen = reinterpret_cast<unsigned*>(shared + n);    // one bit per slot
+  const int mask = (1 << c.page_shift) - 1;
+  for (int i = threadIdx.x; i < (c.n_slots + 31) / 32; i += kCacheThreads) seen[i] = 0;
+  __syncthreads();
+  int need = 0, bad = 0;
+  for (int i0 = 0; i0 < n; i0 += kCacheThreads) {
+    const int i = i0 + threadIdx.x;
+    int want = 0;
+    if (i < n) {
+      const int a = parents[i], b = children[i];
+      if (a < 0 || a >= c.n_slots || b < 0 || b >= c.n_slots) {
+        bad |= 2;
+      } else {
+        const unsigned bit = 1u << (b & 31);
+        const int len = c.lens[a];
+        const int last = len >> c.page_shift;
+        if (c.lens[b] != 0 || (atomicOr(seen + b / 32, bit) & bit)) bad |= 4;
+        if (len < 0 || (static_cast<long long>(len) + mask) >> c.page_shift > c.table_width) {
+          bad |= 1;
+        } else {
+          want = (len & mask) != 0;
+          if (want && (c.tables[a * c.table_stride + last] < 0 || c.tables[a * c.table_stride + last] >= c.n_pages)) bad |= 1;
+        }
+        scratch[1 + 2 * i] = len;
+        scratch[2 + 2 * i] = -1;
+      }
+    }
+    int total;
+    const int before = block_scan(want, &total);
+    if (i < n) first[i] = need + before;
+    need += total;
+  }
+  bad = __syncthreads_or(bad & 2) ? -2 : (__syncthreads_or(bad & 4) ? -3 : (__syncthreads_or(bad & 1) ? -1 : 0));
+  const int found = bad ? 0 : count_free(c.refs, c.n_pages, need);
+  const bool go = !bad && found >= need;
+  if (threadIdx.x == 0) {
+    *status = bad ? bad : max(need - found, 0);
+    scratch[0] = go;
+  }
+  if (!go) return;
+  __syncthreads();
+  // The k-th new page belongs to the pair i with first[i] = k that wants one:
+  // the last pair whose first is <= k.
+  take_free(c.refs, c.n_pages, need, [&](int k, int p) { scratch[2 + 2 * last_at_most(first, n, k)] = p; });
+}
+
+// Carries the fork out: block (i, y) copies its share of the used rows of pair
+// i's partial page (layer and K or V by y); y = 0 also writes the child's
+// table row and counts the shared pages.
+__global__ void __launch_bounds__(256)
+    cache_fork_kernel(const CacheParams c, const int* parents, const int* children, const int* scratch) {
+  if (!scratch[0]) return;
+  const int i = blockIdx.x;
+  const int a = parents[i], b = children[i], len = scratch[1 + 2 * i], fresh = scratch[2 + 2 * i];
+  const int full = len >> c.page_shift, rows = len & ((1 << c.page_shift) - 1);
+  const int* from = c.tables + a * c.table_stride;
+  int* to = c.tables + b * c.table_stride;
+  if (blockIdx.y == 0) {
+    for (int j = threadIdx.x; j < full; j += blockDim.x) {
+      const int p = from[j];
+      to[j] = p;
+      if (p >= 0 && p < c.n_pages) atomicAdd(c.refs + p, 1);
+    }
+    if (threadIdx.x == 0) {
+      if (rows) to[full] = fresh;
+      c.lens[b] = len;
+    }
+  }
+  if (!rows) return;
+  const int src = from[full];
+  const int layer = blockIdx.y >> 1;
+  const bool is_v = blockIdx.y & 1;
+  uint8_t* pool = (is_v ? c.v + layer * c.v_layer : c.k + layer * c.k_layer);
+  const long long stride = is_v ? c.v_stride : c.k_stride;
+  const int head_bytes = c.row_bytes << c.page_shift, used = rows * c.row_bytes;
+  for (int h = 0; h < c.kv_heads; ++h)
+    copy_block(pool + fresh * stride + static_cast<long long>(h) * head_bytes,
+               pool + src * stride + static_cast<long long>(h) * head_bytes, used);
+}
+
+// Plan of compact, n = number of live pages: the k-th live page with index >=
+// n goes to the k-th free index below n.  scratch: [0] moves, [1] n, then
+// rank[n_pages] (k of a moving page), src[n_pages], dst[n_pages].
+__global__ void __launch_bounds__(kCacheThreads) cache_compact_plan_kernel(const CacheParams c, int* scratch, int* live) {
+  int mine = 0;
+  for (int p = threadIdx.x; p < c.n_pages; p += kCacheThreads) mine += c.refs[p] > 0;
+  int n;
+  block_scan(mine, &n);
+  int* rank = scratch + 2;
+  int* src = rank + c.n_pages;
+  int* dst = src + c.n_pages;
+  int holes = 0, moves = 0;
+  for (int p0 = 0; p0 < c.n_pages; p0 += kCacheThreads) {
+    const int p = p0 + threadIdx.x;
+    const bool on = p < c.n_pages && c.refs[p] > 0;
+    const bool hole = p < n && !on, move = p >= n && on;
+    int total;
+    const int both = block_scan((hole ? 1 : 0) + (move ? 1 << 16 : 0), &total);
+    if (hole) dst[holes + (both & 0xffff)] = p;
+    if (move) {
+      rank[p] = moves + (both >> 16);
+      src[rank[p]] = p;
+    }
+    holes += total & 0xffff;
+    moves += total >> 16;
+  }
+  if (threadIdx.x == 0) {
+    scratch[0] = moves;
+    scratch[1] = n;
+    *live = n;
+  }
+}
+
+// Carries the compaction out.  Sources (index >= n) and destinations (< n) are
+// disjoint, so the moves need no order.
+__global__ void __launch_bounds__(512) cache_compact_kernel(const CacheParams c, const int* scratch) {
+  const int moves = scratch[0], n = scratch[1];
+  const int* rank = scratch + 2;
+  const int* src = rank + c.n_pages;
+  const int* dst = src + c.n_pages;
+  const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
+  const long long at = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+  if (moves > 0)
+    for (long long x = at; x < static_cast<long long>(c.n_slots) * c.table_width; x += step) {
+      int* e = c.tables + x / c.table_width * c.table_stride + x % c.table_width;
+      const int p = *e;
+      if (p >= n && p < c.n_pages) *e = dst[rank[p]];
+    }
+  for (long long k = at; k < moves; k += step) {
+    c.refs[dst[k]] = c.refs[src[k]];
+    c.refs[src[k]] = 0;
+  }
+  const int page_bytes = c.kv_heads * (c.row_bytes << c.page_shift);
+  const int parts = 2 * c.layers;
+  for (long long job = blockIdx.x; job < static_cast<long long>(moves) * parts; job += gridDim.x) {
+    const int k = static_cast<int>(job / parts), part = static_cast<int>(job % parts), layer = part >> 1;
+    uint8_t* pool = part & 1 ? c.v + layer * c.v_layer : c.k + layer * c.k_layer;
+    const long long stride = part & 1 ? c.v_stride : c.k_stride;
+    copy_block(pool + dst[k] * stride, pool + src[k] * stride, page_bytes);
+  }
+}
+
+// Copies whole pages src[i] -> dst[i] of every layer (a pair with an index outside the pool is skipped).
+__global__ void __launch_bounds__(512)
+    cache_copy_pages_kernel(const CacheParams c, const int* src, const int* dst, int n) {
+  const int page_bytes = c.kv_heads * (c.row_bytes << c.page_shift);
+  const int parts = 2 * c.layers;
+  for (long long job = blockIdx.x; job < static_cast<long long>(n) * parts; job += gridDim.x) {
+    const int k = static_cast<int>(job / parts), part = static_cast<int>(job % parts), layer = part >> 1;
+    const int a = src[k], b = dst[k];
+    if (a < 0 || a >= c.n_pages || b < 0 || b >= c.n_pages || a == b) continue;
+    uint8_t* pool = part & 1 ? c.v + layer * c.v_layer : c.k + layer * c.k_layer;
+    const long long stride = part & 1 ? c.v_stride : c.k_stride;
+    copy_block(pool + b * stride, pool + a * stride, page_bytes);
+  }
+}
+
+}  // namespace tt

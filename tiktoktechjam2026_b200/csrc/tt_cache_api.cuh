@@ -1,0 +1,316 @@
+// Host side of the paged K/V cache entry points (tt_cache_*, tt_paged_attention).
+// Included once, at the end of tt_b200.cu, whose launch helpers it uses.
+#pragma once
+
+#include <exception>
+
+#include "tt_cache.cuh"
+#include "tt_paged_attn.cuh"
+
+namespace {
+
+// No C++ exception leaves a C entry point.
+template <typename F>
+int guarded(F f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return fail(TT_ERR_LAUNCH, "%s", e.what());
+  } catch (...) {
+    return fail(TT_ERR_LAUNCH, "unknown C++ exception");
+  }
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Checks the fields of a cache that every call uses, plus what `values` (K and
+// V) and `counts` (refs) ask for, and fills the kernels' parameters.
+int cache_params(const tt_kv_cache* c, bool values, bool counts, CacheParams* out) {
+  if (!c || !c->tables || !c->lens || (counts && !c->refs) || (values && (!c->k || !c->v)))
+    return fail(TT_ERR_ARG, "null cache field");
+  if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128 && c->page != 256)
+    return fail(TT_ERR_UNSUPPORTED, "page %d not in {16, 32, 64, 128, 256}", c->page);
+  if (c->n_slots <= 0 || c->table_width <= 0 || c->n_pages <= 0 || c->table_stride < c->table_width)
+    return fail(TT_ERR_SHAPE, "invalid slots, table width, table stride or pages (%d, %d, %lld, %d)", c->n_slots,
+                c->table_width, static_cast<long long>(c->table_stride), c->n_pages);
+  if (static_cast<long long>(c->table_width) * c->page > 0x7fffffffLL)
+    return fail(TT_ERR_SHAPE, "table rows of %d pages of %d tokens pass 2^31 tokens", c->table_width, c->page);
+  memset(out, 0, sizeof(*out));
+  out->tables = c->tables;
+  out->table_stride = c->table_stride;
+  out->lens = c->lens;
+  out->refs = c->refs;
+  out->n_pages = c->n_pages;
+  out->n_slots = c->n_slots;
+  out->table_width = c->table_width;
+  while ((1 << out->page_shift) < c->page) ++out->page_shift;
+  if (!values) return TT_OK;
+  if (c->head_dim != 16 && c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(TT_ERR_UNSUPPORTED, "stored head_dim %d not in {16, 32, 64, 128, 256}", c->head_dim);
+  if (c->layers <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535)
+    return fail(TT_ERR_SHAPE, "invalid layers or kv_heads (%d, %d)", c->layers, c->kv_heads);
+  const long long page_elems = static_cast<long long>(c->kv_heads) * c->page * c->head_dim;
+  if (page_elems > 0x3fffffffLL) return fail(TT_ERR_SHAPE, "a page of %lld values is too large", page_elems);
+  if (!aligned16(c->k) || !aligned16(c->v) ||
+      (c->k_page_stride | c->v_page_stride | c->k_layer_stride | c->v_layer_stride) % 8 != 0)
+    return fail(TT_ERR_ALIGN, "pools must be 16-byte aligned and their strides multiples of 8 elements");
+  if (c->k_page_stride < page_elems || c->v_page_stride < page_elems)
+    return fail(TT_ERR_SHAPE, "page strides are smaller than a page (%lld values)", page_elems);
+  out->k = static_cast<uint8_t*>(c->k);
+  out->v = static_cast<uint8_t*>(c->v);
+  out->k_layer = c->k_layer_stride * 2;
+  out->v_layer = c->v_layer_stride * 2;
+  out->k_stride = c->k_page_stride * 2;
+  out->v_stride = c->v_page_stride * 2;
+  out->layers = c->layers;
+  out->kv_heads = c->kv_heads;
+  out->row_bytes = c->head_dim * 2;
+  return TT_OK;
+}
+
+// ---------------------------------------------------------------- attention
+// Units that a worker takes at least: fewer would cost more in joining than
+// the shorter pieces save.
+constexpr long long kRowsMinUnits = 2;
+
+template <int HD>
+size_t paged_part_bytes(int sm_count) {
+  return 2ull * sm_count * PagedRowsLayout<HD>::WARPS * paged_slot_floats<16, HD>() * sizeof(float);
+}
+
+int paged_workspace(int hd, int sm_count, size_t* bytes) {
+  switch (hd) {
+    case 8:
+    case 16: *bytes = paged_part_bytes<16>(sm_count); return TT_OK;
+    case 32: *bytes = paged_part_bytes<32>(sm_count); return TT_OK;
+    case 64: *bytes = paged_part_bytes<64>(sm_count); return TT_OK;
+    case 128: *bytes = paged_part_bytes<128>(sm_count); return TT_OK;
+    case 256: *bytes = paged_part_bytes<256>(sm_count); return TT_OK;
+    default: return fail(TT_ERR_UNSUPPORTED, "head_dim %d not in {8, 16, 32, 64, 128, 256}", hd);
+  }
+}
+
+template <typename T, int HD>
+int launch_paged(PagedParams p, int max_rows, int sm_count, cudaStream_t stream) {
+  using L = PagedRowsLayout<HD>;
+  (void)max_rows;
+  auto kern = paged_rows_kernel<T, HD>;
+  if (int rc = prepare_kernel(kern, L::SMEM)) return rc;
+  p.row_lo = 0;
+  p.row_hi = 0x7fffffff;
+  p.n_workers = sm_count * L::WARPS;
+  launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, p, kRowsMinUnits);
+  if (int rc = after_launch("paged attention")) return rc;
+  launch_kernel(paged_join_kernel<T, HD, L::TK, 16, 16, 256>, p.n_workers - 1, 256, 0, stream, p, 16, kRowsMinUnits);
+  return after_launch("paged attention join");
+}
+
+template <typename T>
+int launch_paged_t(const PagedParams& p, int hd, int max_rows, int sm_count, cudaStream_t stream) {
+  switch (hd) {
+    case 16: return launch_paged<T, 16>(p, max_rows, sm_count, stream);
+    case 32: return launch_paged<T, 32>(p, max_rows, sm_count, stream);
+    case 64: return launch_paged<T, 64>(p, max_rows, sm_count, stream);
+    case 128: return launch_paged<T, 128>(p, max_rows, sm_count, stream);
+    default: return launch_paged<T, 256>(p, max_rows, sm_count, stream);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int tt_cache_reserve(const tt_kv_cache* cache, const int* cu_q, const int* slots, int batch, int* status,
+                     void* stream) {
+  return guarded([&]() -> int {
+    DeviceState* ds;
+    if (int rc = current_device_state(&ds)) return rc;
+    CacheParams c;
+    if (int rc = cache_params(cache, false, true, &c)) return rc;
+    if (!status || !cu_q) return fail(TT_ERR_ARG, "null argument");
+    if (batch < 0 || batch > kCacheMaxBatch)
+      return fail(TT_ERR_SHAPE, "batch %d outside 0 .. %d", batch, kCacheMaxBatch);
+    if (int rc = prepare_kernel(cache_reserve_kernel, kCacheMaxBatch * 4)) return rc;
+    launch_kernel(cache_reserve_kernel, 1, kCacheThreads, static_cast<size_t>(batch) * 4,
+                  static_cast<cudaStream_t>(stream), c, cu_q, slots, batch, status);
+    return after_launch("cache reserve");
+  });
+}
+
+int tt_cache_append(const tt_kv_cache* cache, const void* k, const int64_t* k_strides, const void* v,
+                    const int64_t* v_strides, int n_tokens, const int* cu_q, const int* slots, int batch,
+                    void* stream) {
+  return guarded([&]() -> int {
+    DeviceState* ds;
+    if (int rc = current_device_state(&ds)) return rc;
+    CacheParams c;
+    if (int rc = cache_params(cache, true, false, &c)) return rc;
+    if ((n_tokens > 0 && (!k || !v)) || !k_strides || !v_strides || !cu_q) return fail(TT_ERR_ARG, "null argument");
+    if (n_tokens < 0 || batch < 0) return fail(TT_ERR_SHAPE, "invalid n_tokens or batch (%d, %d)", n_tokens, batch);
+    if (n_tokens == 0 || batch == 0) return TT_OK;
+    AppendSrc src[2];
+    const void* ptr[2] = {k, v};
+    const int64_t* st[2] = {k_strides, v_strides};
+    for (int i = 0; i < 2; ++i) {
+      const char* name = i ? "v" : "k";
+      src[i] = {static_cast<const uint16_t*>(ptr[i]), st[i][0], st[i][1], st[i][2]};
+      if (st[i][2] == 1) {
+        if (!aligned16(ptr[i]) || st[i][0] % 8 != 0 || st[i][1] % 8 != 0)
+          return fail(TT_ERR_ALIGN, "%s rows must be 16-byte aligned", name);
+      } else if (st[i][0] != 1) {
+        return fail(TT_ERR_ARG, "%s must be dense in its features or in its tokens", name);
+      }
+    }
+    const int smem = c.row_bytes / 2 * (kAppendTokens + 2) * 2;
+    if (int rc = prepare_kernel(cache_append_kernel, smem)) return rc;
+    launch_kernel(cache_append_kernel, dim3((n_tokens + kAppendTokens - 1) / kAppendTokens, c.kv_heads),
+                  kAppendThreads, smem, static_cast<cudaStream_t>(stream), c, src[0], src[1], cu_q, slots, batch,
+                  n_tokens);
+    return after_launch("cache append");
+  });
+}
+
+int tt_cache_release(const tt_kv_cache* cache, const int* slots, int n, int window, int sinks, void* stream) {
+  return guarded([&]() -> int {
+    DeviceState* ds;
+    if (int rc = current_device_state(&ds)) return rc;
+    CacheParams c;
+    if (int rc = cache_params(cache, false, true, &c)) return rc;
+    if (window < 0 || sinks < 0) return fail(TT_ERR_ARG, "window and sinks must not be negative (%d, %d)", window, sinks);
+    if (n < 0 || (!slots && n > c.n_slots)) return fail(TT_ERR_SHAPE, "invalid slot count %d", n);
+    if (n == 0) return TT_OK;
+    launch_kernel(cache_release_kernel, n, 256, 0, static_cast<cudaStream_t>(stream), c, slots, n, window, sinks);
+    return after_launch("cache release");
+  });
+}
+
+int tt_cache_fork(const tt_kv_cache* cache, const int* parents, const int* children, int n, int* scratch, int* status,
+                  void* stream) {
+  return guarded([&]() -> int {
+    DeviceState* ds;
+    if (int rc = current_device_state(&ds)) return rc;
+    CacheParams c;
+    if (int rc = cache_params(cache, true, true, &c)) return rc;
+    if ((n > 0 && (!parents || !children)) || !scratch || !status) return fail(TT_ERR_ARG, "null argument");
+    constexpr int kMaxBits = kCacheMaxSlots / 32 * 4;
+    if (n < 0 || n > kCacheMaxBatch || c.n_slots > kCacheMaxSlots || c.layers > 32767)
+      return fail(TT_ERR_SHAPE, "fork takes at most %d pairs, %d slots and 32767 layers (got %d, %d, %d)",
+                  kCacheMaxBatch, kCacheMaxSlots, n, c.n_slots, c.layers);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (int rc = prepare_kernel(cache_fork_plan_kernel, kCacheMaxBatch * 4 + kMaxBits)) return rc;
+    launch_kernel(cache_fork_plan_kernel, 1, kCacheThreads, static_cast<size_t>(n) * 4 + (c.n_slots + 31) / 32 * 4, s, c,
+                  parents, children, n, scratch, status);
+    if (int rc = after_launch("cache fork plan")) return rc;
+    if (n == 0) return TT_OK;
+    launch_kernel(cache_fork_kernel, dim3(n, 2 * c.layers), 256, 0, s, c, parents, children,
+                  static_cast<const int*>(scratch));
+    return after_launch("cache fork");
+  });
+}
+
+int tt_cache_compact(const tt_kv_cache* cache, int* scratch, int* live, void* stream) {
+  return guarded([&]() -> int {
+    DeviceState* ds;
+    if (int rc = current_device_state(&ds)) return rc;
+    CacheParams c;
+    if (int rc = cache_params(cache, true, true, &c)) return rc;
+    if (!scratch || !live) return fail(TT_ERR_ARG, "null argument");
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    launch_kernel(cache_compact_plan_kernel, 1, kCacheThreads, 0, s, c, scratch, live);
+    if (int rc = after_launch("cache compact plan")) return rc;
+    launch_kernel(cache_compact_kernel, 4 * ds->sm_count, 512, 0, s, c, static_cast<const int*>(scratch));
+    return after_launch("cache compact");
+  });
+}
+
+int tt_cache_copy_pages(const tt_kv_cache* cache, const int* src, const int* dst, int n, void* stream) {
+  return guarded([&]() -> int {
+    DeviceState* ds;
+    if (int rc = current_device_state(&ds)) return rc;
+    CacheParams c;
+    if (int rc = cache_params(cache, true, false, &c)) return rc;
+    if (n > 0 && (!src || !dst)) return fail(TT_ERR_ARG, "null argument");
+    if (n < 0) return fail(TT_ERR_SHAPE, "invalid page count %d", n);
+    if (n == 0) return TT_OK;
+    launch_kernel(cache_copy_pages_kernel, 4 * ds->sm_count, 512, 0, static_cast<cudaStream_t>(stream), c, src, dst, n);
+    return after_launch("cache copy pages");
+  });
+}
+
+int tt_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int max_q_len, size_t* bytes) {
+  return guarded([&]() -> int {
+    DeviceState* ds;
+    if (int rc = current_device_state(&ds)) return rc;
+    if (!bytes) return fail(TT_ERR_ARG, "null argument");
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0)
+      return fail(TT_ERR_SHAPE, "heads %d must be a multiple of kv_heads %d", heads, kv_heads);
+    (void)max_q_len;
+    return paged_workspace(head_dim, ds->sm_count, bytes);
+  });
+}
+
+int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                       const int* cu_q, const int* slots, int batch, void* out, int n_tokens, int heads, int head_dim,
+                       int is_bf16, float scale, int window, int sinks, int max_q_len, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    DeviceState* ds;
+    if (int rc = current_device_state(&ds)) return rc;
+    CacheParams c;
+    if (int rc = cache_params(cache, true, false, &c)) return rc;
+    if ((n_tokens > 0 && (!q || !out)) || !cu_q || !workspace) return fail(TT_ERR_ARG, "null argument");
+    if (n_tokens < 0 || batch < 0 || heads <= 0 || heads % c.kv_heads != 0 || heads / c.kv_heads > 128)
+      return fail(TT_ERR_SHAPE, "invalid sizes (n_tokens %d, batch %d, heads %d, kv_heads %d)", n_tokens, batch, heads,
+                  c.kv_heads);
+    if (window < 0 || sinks < 0) return fail(TT_ERR_ARG, "window and sinks must not be negative (%d, %d)", window, sinks);
+    size_t need = 0;
+    if (int rc = paged_workspace(head_dim, ds->sm_count, &need)) return rc;
+    if (stored_head_dim(head_dim) != cache->head_dim)
+      return fail(TT_ERR_SHAPE, "head_dim %d is stored %d wide, the cache has %d", head_dim, stored_head_dim(head_dim),
+                  cache->head_dim);
+    if (workspace_bytes < need)
+      return fail(TT_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || q_token_stride % 8 != 0 || q_head_stride % 8 != 0)
+      return fail(TT_ERR_ALIGN, "q, out and workspace must be 16-byte aligned, q's strides multiples of 8");
+    const int group = heads / c.kv_heads;
+    if (static_cast<long long>(n_tokens) * group > 0x7fffffffLL) return fail(TT_ERR_SHAPE, "too many query rows");
+    if (n_tokens == 0) return TT_OK;
+    PagedParams p;
+    memset(&p, 0, sizeof(p));
+    p.q = q;
+    p.q_token = q_token_stride;
+    p.q_head = q_head_stride;
+    p.k_pages = cache->k;
+    p.v_pages = cache->v;
+    p.k_stride = cache->k_page_stride;
+    p.v_stride = cache->v_page_stride;
+    p.tables = c.tables;
+    p.table_stride = c.table_stride;
+    p.lens = c.lens;
+    p.cu_q = cu_q;
+    p.slots = slots;
+    p.out = out;
+    p.part = static_cast<float*>(workspace);
+    p.n_tokens = n_tokens;
+    p.batch = batch;
+    p.n_slots = c.n_slots;
+    p.heads = heads;
+    p.kv_heads = c.kv_heads;
+    p.group = group;
+    p.n_pages = c.n_pages;
+    p.page_shift = c.page_shift;
+    p.table_width = c.table_width;
+    p.window = window;
+    p.sinks = sinks;
+    p.out_hd = head_dim;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.err = ds->err;
+    p.timeout_ns = g_timeout_ns.load();
+    const int max_rows = (max_q_len > 0 && max_q_len < n_tokens ? max_q_len : n_tokens) * group;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return is_bf16 ? launch_paged_t<__nv_bfloat16>(p, cache->head_dim, max_rows, ds->sm_count, s)
+                   : launch_paged_t<__half>(p, cache->head_dim, max_rows, ds->sm_count, s);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,589 @@
+// Attention of a chunk of new tokens over a paged K/V cache, with grouped KV
+// heads, an optional sliding window and a few first tokens that stay visible:
+// parameters, work schedule and the kernel for short chunks (sm_100a).
+//
+// Sequence b has the query rows cu_q[b] .. cu_q[b+1] of its T new tokens and L
+// = lens[slot] keys, the new ones included.  Query j stands at t = L - T + j
+// and sees key u iff 0 <= u <= t and (no window, or t - u < window, or u <
+// sinks):
+//   o = sum_u 2^(s_u - m) v_u / sum_u 2^(s_u - m),  s_u = (q . k_u) scale log2 e.
+// A row that sees no key (t < 0) is zero, and so is a row of no sequence.
+//
+// Work is measured in units of one key tile of one item (a tile of query rows
+// of one sequence and KV head).  All units of the call form one line, cut into
+// equal pieces, one per worker: a worker's piece may begin and end inside an
+// item, so a single long sequence and a ragged batch both fill the GPU.  An
+// item that lies in one piece is finished by its worker; the parts of an item
+// that was cut (O unnormalised, m, l, in FP32) go to the workspace and are
+// joined by paged_join_kernel, always in worker order, so results do not
+// depend on timing.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "tt_ptx.cuh"
+
+namespace tt {
+
+struct PagedParams {
+  const void* q;               // [n_tokens, heads, HD], element strides below, last dimension dense
+  long long q_token, q_head;
+  const void* k_pages;         // [n_pages, kv_heads, page, HD], pages k_stride elements apart
+  const void* v_pages;
+  long long k_stride, v_stride;
+  const int* tables;           // [n_slots, table_width], rows table_stride apart; < 0: no page
+  long long table_stride;
+  const int* lens;             // [n_slots]
+  const int* cu_q;             // [batch + 1]
+  const int* slots;            // [batch], or nullptr: slot b is sequence b
+  void* out;                   // [n_tokens, heads * out_hd]
+  float* part;                 // parts of cut items
+  int n_tokens, batch, n_slots, heads, kv_heads, group;
+  int n_pages, page_shift, table_width;
+  int window, sinks;           // window 0: none
+  int out_hd;
+  int row_lo, row_hi;          // this launch serves sequences of row_lo .. row_hi query rows (T * group)
+  int n_workers;
+  float scale_log2;
+  unsigned int* err;
+  unsigned long long timeout_ns;
+};
+
+struct PagedSeq {
+  int q0, T, L, slot;
+};
+
+// Sequence b with every field brought into range: rows outside q, a slot or a
+// length that does not exist become an empty sequence or an empty cache.
+__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
+  PagedSeq s;
+  s.q0 = min(max(p.cu_q[b], 0), p.n_tokens);
+  s.T = max(min(p.cu_q[b + 1], p.n_tokens) - s.q0, 0);
+  s.slot = p.slots ? p.slots[b] : b;
+  const bool ok = s.slot >= 0 && s.slot < p.n_slots;
+  s.slot = ok ? s.slot : 0;
+  const long long room = static_cast<long long>(p.table_width) << p.page_shift;
+  const int len = ok ? p.lens[s.slot] : 0;
+  s.L = static_cast<int>(min(static_cast<long long>(max(len, 0)), room));
+  return s;
+}
+
+// One item: RPT query rows (row = token * group + head of the group) of one
+// sequence, and the key tiles that some row of it can see.  With a window the
+// tiles are [0, n_sink) and [w_tile, ...); tile(i) maps the i-th of n.
+template <int TK>
+struct PagedItem {
+  int r0, rows, p0, p1;  // first row, rows, positions of the first and last row's token
+  int n, n_sink, w_tile;
+  __device__ __forceinline__ void set(const PagedParams& p, const PagedSeq& s, int qt, int rpt) {
+    r0 = qt * rpt;
+    rows = min(rpt, s.T * p.group - r0);
+    p0 = s.L - s.T + r0 / p.group;
+    p1 = s.L - s.T + (r0 + rows - 1) / p.group;
+    const int total = p1 < 0 ? 1 : p1 / TK + 1;  // an item of rows that see nothing keeps one tile, wholly masked
+    n_sink = total;
+    w_tile = total;
+    n = total;
+    if (p.window > 0) {
+      const int first = max(p0 - p.window + 1, 0);
+      const int ns = (min(p.sinks, first) + TK - 1) / TK;
+      const int wt = first / TK;
+      if (ns < wt) {
+        n_sink = ns;
+        w_tile = wt;
+        n = ns + max(total - wt, 0);
+        if (n == 0) n = 1;
+      }
+    }
+  }
+  __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : i - n_sink + w_tile; }
+  // Whether every row sees every key of [k0, k0 + TK).
+  __device__ __forceinline__ bool whole(const PagedParams& p, int k0) const {
+    return k0 + TK - 1 <= p0 && (p.window == 0 || k0 > p1 - p.window || k0 + TK <= p.sinks);
+  }
+};
+
+__device__ __forceinline__ int paged_q_tiles(const PagedParams& p, const PagedSeq& s, int rpt) {
+  const int rows = s.T * p.group;
+  return rows >= p.row_lo && rows <= p.row_hi ? (rows + rpt - 1) / rpt : 0;
+}
+
+// Units of sequence b for one KV head.
+template <int TK>
+__device__ __forceinline__ long long paged_head_units(const PagedParams& p, const PagedSeq& s, int rpt) {
+  const int nq = paged_q_tiles(p, s, rpt);
+  long long u = 0;
+  PagedItem<TK> it;
+  for (int qt = 0; qt < nq; ++qt) {
+    it.set(p, s, qt, rpt);
+    u += it.n;
+  }
+  return u;
+}
+
+// Walks the units of one worker's piece: sequence, KV head, query tile, tile.
+template <int TK>
+struct PagedCursor {
+  int b, kvh, qt, nq, i;
+  PagedSeq s;
+  PagedItem<TK> it;
+  __device__ __forceinline__ void open(const PagedParams& p, int rpt) {  // enters sequence b, or the next with work
+    while (b < p.batch) {
+      s = paged_seq(p, b);
+      nq = paged_q_tiles(p, s, rpt);
+      if (nq > 0) {
+        it.set(p, s, 0, rpt);
+        return;
+      }
+      ++b;
+    }
+  }
+  // Places the cursor `off` units into sequence b.
+  __device__ __forceinline__ void seek(const PagedParams& p, int b_, long long off, int rpt) {
+    b = b_;
+    s = paged_seq(p, b);
+    nq = paged_q_tiles(p, s, rpt);
+    const long long per_head = paged_head_units<TK>(p, s, rpt);
+    kvh = static_cast<int>(off / per_head);
+    off -= kvh * per_head;
+    qt = 0;
+    it.set(p, s, 0, rpt);
+    while (off >= it.n) {
+      off -= it.n;
+      it.set(p, s, ++qt, rpt);
+    }
+    i = static_cast<int>(off);
+  }
+  __device__ __forceinline__ void next_item(const PagedParams& p, int rpt) {
+    i = 0;
+    if (++qt < nq) {
+      it.set(p, s, qt, rpt);
+      return;
+    }
+    qt = 0;
+    if (++kvh < p.kv_heads) {
+      it.set(p, s, 0, rpt);
+      return;
+    }
+    kvh = 0;
+    ++b;
+    open(p, rpt);
+  }
+};
+
+// Where a worker's piece begins: sequence and units into it (b < 0: no work).
+struct PagedStart {
+  int b;
+  long long off;
+};
+
+// Block-wide: total units, units per worker, and the start of the workers
+// first_worker .. first_worker + NW - 1 (fewer than 32).  Every thread takes part.
+template <int TK, int NW, int THREADS>
+__device__ __forceinline__ void paged_schedule(const PagedParams& p, int rpt, long long min_units, int first_worker,
+                                               PagedStart* starts, long long* total, long long* per) {
+  constexpr int NWARPS = THREADS / 32;
+  __shared__ long long warp_sum[NWARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  long long sum = 0;
+  for (int b = tid; b < p.batch; b += THREADS) sum += paged_head_units<TK>(p, paged_seq(p, b), rpt) * p.kv_heads;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  if (lane == 0) warp_sum[warp] = sum;
+  if (tid < NW) starts[tid].b = -1;
+  __syncthreads();
+  long long all = 0;
+  for (int w = 0; w < NWARPS; ++w) all += warp_sum[w];
+  const long long each = max((all + p.n_workers - 1) / p.n_workers, min_units);
+  *total = all;
+  *per = each;
+  long long carry = 0;
+  for (int b0 = 0; b0 < p.batch && all > 0; b0 += THREADS) {
+    const int b = b0 + tid;
+    const long long u = b < p.batch ? paged_head_units<TK>(p, paged_seq(p, b), rpt) * p.kv_heads : 0;
+    long long inc = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(~0u, inc, o);
+      if (lane >= o) inc += v;
+    }
+    __syncthreads();  // warp_sum is reread above and in the previous round
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    long long before = carry;
+    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    for (int w = 0; w < NWARPS; ++w) carry += warp_sum[w];
+    const long long lo = before + inc - u, hi = before + inc;
+    for (int w = 0; w < NW; ++w) {
+      const long long start = (first_worker + w) * each;
+      if (start >= lo && start < hi) starts[w] = {b, start - lo};
+    }
+  }
+  __syncthreads();
+}
+
+// Zeros the rows of q that belong to no sequence (before cu_q[0], from cu_q[batch] on).
+__device__ __forceinline__ void paged_zero_outside(const PagedParams& p, int threads) {
+  const int lo = p.batch > 0 ? min(max(p.cu_q[0], 0), p.n_tokens) : 0;
+  const int hi = p.batch > 0 ? min(max(p.cu_q[p.batch], lo), p.n_tokens) : 0;
+  const long long row = static_cast<long long>(p.heads) * p.out_hd / 8;  // 16-byte pieces
+  const long long n = (lo + p.n_tokens - hi) * row;
+  uint4* out = static_cast<uint4*>(p.out);
+  for (long long i = blockIdx.x * static_cast<long long>(threads) + threadIdx.x; i < n;
+       i += static_cast<long long>(gridDim.x) * threads) {
+    const long long at = i < lo * row ? i : i - lo * row + hi * row;
+    out[at] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <typename T>
+struct Pair16;  // two 16-bit values in a register, and the MMA on them
+template <>
+struct Pair16<__half> {
+  static constexpr bool kBf16 = false;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_half2(lo, hi); }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <>
+struct Pair16<__nv_bfloat16> {
+  static constexpr bool kBf16 = true;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Parts of cut items.  Worker w owns the slots 2w (its piece begins inside an
+// item) and 2w + 1 (an item that begins in its piece and goes on past it).
+// A slot holds ROWS x HD of O, then ROWS of m and ROWS of l.
+// ---------------------------------------------------------------------------
+template <int ROWS, int HD>
+__host__ __device__ constexpr long long paged_slot_floats() {
+  return static_cast<long long>(ROWS) * (HD + 2);
+}
+
+// Joins the parts of the item that the start of worker c cuts, if c is the
+// first worker to start inside it: with M = max_i m_i,
+//   O = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
+// One block per (worker, RB rows of the item); a thread per two features.
+template <typename T, int HD, int TK, int ROWS, int RB, int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_join_kernel(const PagedParams p, int rpt, long long min_units) {
+  __shared__ PagedStart start;
+  long long total, per;
+  const int c = blockIdx.x + 1;  // worker 0 starts at an item's beginning
+  pdl_wait();
+  pdl_trigger();
+  paged_schedule<TK, 1, THREADS>(p, rpt, min_units, c, &start, &total, &per);
+  if (start.b < 0) return;
+  PagedCursor<TK> cur;
+  cur.seek(p, start.b, start.off, rpt);
+  if (cur.i == 0 || cur.i > per) return;  // starts with the item, or an earlier worker starts inside it
+  const long long end = static_cast<long long>(c) * per - cur.i + cur.it.n;  // one past the item's last unit
+  const int n_after = static_cast<int>((end - 1) / per) - c + 1;             // workers c .. that hold a part
+  constexpr long long SLOT = paged_slot_floats<ROWS, HD>();
+  const float* first = p.part + (2ll * (c - 1) + 1) * SLOT;
+  const float* rest = p.part + 2ll * c * SLOT;  // then every 2 SLOT
+  constexpr int TPR = HD / 2;                   // threads of one row
+  for (int x = threadIdx.x; x < RB * TPR; x += THREADS) {
+    const int row = blockIdx.y * RB + x / TPR, d = x % TPR * 2;
+    if (row >= cur.it.rows || d >= p.out_hd) continue;
+    const int o_at = row * HD + d, m_at = ROWS * HD + row, l_at = m_at + ROWS;
+    float m = first[m_at];
+    for (int k = 0; k < n_after; ++k) m = fmaxf(m, rest[2 * SLOT * k + m_at]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float w = ex2_approx(first[m_at] - base);
+    float l = first[l_at] * w;
+    const float2 o0 = *reinterpret_cast<const float2*>(first + o_at);
+    float a0 = o0.x * w, a1 = o0.y * w;
+    for (int k = 0; k < n_after; ++k) {
+      const float* s = rest + 2 * SLOT * k;
+      w = ex2_approx(s[m_at] - base);
+      l = fmaf(s[l_at], w, l);
+      const float2 o = *reinterpret_cast<const float2*>(s + o_at);
+      a0 = fmaf(o.x, w, a0);
+      a1 = fmaf(o.y, w, a1);
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int r = cur.it.r0 + row, tok = cur.s.q0 + r / p.group, h = cur.kvh * p.group + r % p.group;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) +
+                                                (static_cast<long long>(tok) * p.heads + h) * p.out_hd + d);
+    *dst = Pair16<T>::pack(a0 * inv, a1 * inv);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Short chunks: at most 16 query rows per item, so the cache is read at most
+// once per 16 rows and the memory system bounds the kernel.  Every warp is a
+// worker of its own with a private ring of NST stages (TK keys and values,
+// 16-byte asynchronous copies), no block-wide synchronisation in the loop:
+//   S = Q K^T (mma.sync m16n8k16, FP32), online softmax on the fragments,
+//   O += P V with P rounded to the cache's type (the A operand's layout is the
+//   accumulator's, so P never leaves registers).
+// Values of keys past the sequence's end are zero-filled by the copy: stale
+// rows of a page never reach the sum.
+// ---------------------------------------------------------------------------
+template <int HD>
+struct PagedRowsLayout {
+  static constexpr int TK = HD >= 128 ? 16 : 2048 / HD;  // keys per tile: 4 KB of K (8 KB at 256 features)
+  static constexpr int WARPS = HD == 256 ? 4 : 8;
+  static constexpr int THREADS = 32 * WARPS;
+  static constexpr int NST = 3;
+  static constexpr int RB = HD * 2;  // bytes of a row
+  static constexpr int TILE = TK * RB;
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int SMEM = WARPS * NST * STAGE + 128;
+  static constexpr int CH = RB / 16;                 // 16-byte pieces of a row
+  static constexpr int RPL = RB >= 128 ? 1 : 128 / RB;  // rows per 128 bytes
+  static constexpr int SWM = CH < 8 ? CH - 1 : 7;
+  static_assert(SMEM <= 232448, "shared memory budget");
+};
+
+// Byte offset of 16-byte piece c of row r: the pieces are permuted so that the
+// same piece of eight consecutive rows falls into eight different bank groups.
+template <int HD>
+__device__ __forceinline__ uint32_t paged_rows_at(int r, int c) {
+  using L = PagedRowsLayout<HD>;
+  return r * L::RB + ((c ^ ((r / L::RPL) & L::SWM)) << 4);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
+    paged_rows_kernel(const PagedParams p, long long min_units) {
+  using L = PagedRowsLayout<HD>;
+  using PT = Pair16<T>;
+  constexpr int TK = L::TK, NST = L::NST, RPT = 16;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ PagedStart starts[L::WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t ring = ((smem_u32(smem_raw) + 127) & ~127u) + warp * NST * L::STAGE;
+  long long total, per;
+  const int worker0 = blockIdx.x * L::WARPS;
+  paged_schedule<TK, L::WARPS, L::THREADS>(p, RPT, min_units, worker0, starts, &total, &per);
+  paged_zero_outside(p, L::THREADS);
+  if (starts[warp].b < 0) return;
+  const int worker = worker0 + warp;
+  const long long begin = worker * per;
+  const int n_units = static_cast<int>(min(per, total - begin));
+
+  PagedCursor<TK> cur, ahead;
+  cur.seek(p, starts[warp].b, starts[warp].off, RPT);
+  ahead = cur;
+
+  // Copies the K and V tile under `ahead` into stage st and moves it on.
+  auto fetch = [&](int st) {
+    const int k0 = ahead.it.tile(ahead.i) * TK;
+    const int* row = p.tables + ahead.s.slot * p.table_stride;
+    const int page_at = (k0 >> p.page_shift) + lane;
+    int page = page_at < p.table_width ? row[page_at] : -1;  // lane i: the i-th page of the tile
+    if (page >= p.n_pages) page = -1;
+    const uint32_t sk = ring + st * L::STAGE, sv = sk + L::TILE;
+#pragma unroll
+    for (int c0 = 0; c0 < TK * L::CH; c0 += 32) {
+      const int c = c0 + lane, r = c / L::CH, ch = c % L::CH;
+      const int key = k0 + r;
+      const int pg = __shfl_sync(~0u, page, (key >> p.page_shift) - (k0 >> p.page_shift));
+      const bool ok = pg >= 0 && key < ahead.s.L;
+      const long long in_page =
+          (static_cast<long long>(ahead.kvh) << p.page_shift) * HD + (key & ((1 << p.page_shift) - 1)) * HD + ch * 8;
+      const long long at = ok ? pg : 0;
+      cp_async_16(sk + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.k_pages) + at * p.k_stride + in_page,
+                  ok ? 16u : 0u);
+      cp_async_16(sv + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.v_pages) + at * p.v_stride + in_page,
+                  ok ? 16u : 0u);
+    }
+    if (++ahead.i == ahead.it.n) ahead.next_item(p, RPT);
+  };
+
+  int fetched = 0;
+  for (; fetched < NST - 1; ++fetched) {
+    if (fetched < n_units) fetch(fetched);
+    cp_async_commit();
+  }
+
+  uint32_t qf[HD / 16][4];
+  float o[HD / 8][4];
+  float m[2], l[2];
+  int pos[2];
+  bool fresh = true;
+  const int seg0 = cur.i;       // the piece begins this far into its first item
+  bool from_start = seg0 == 0;  // the current item's first tile is in this piece
+  for (int u = 0; u < n_units; ++u) {
+    if (fresh) {
+      fresh = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = min(lane / 4 + 8 * h, cur.it.rows - 1) + cur.it.r0;
+        const int tok = r / p.group, head = cur.kvh * p.group + r % p.group;
+        pos[h] = cur.s.L - cur.s.T + tok;
+        const T* src = static_cast<const T*>(p.q) + (cur.s.q0 + tok) * p.q_token + head * p.q_head + lane % 4 * 2;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          qf[kk][h] = *reinterpret_cast<const uint32_t*>(src + kk * 16);
+          qf[kk][2 + h] = *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8);
+        }
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+      }
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    }
+    if (fetched < n_units) fetch(fetched % NST);
+    ++fetched;
+    cp_async_commit();
+    cp_async_wait<NST - 1>();
+    __syncwarp();
+    const uint32_t sk = ring + u % NST * L::STAGE, sv = sk + L::TILE;
+    const int k0 = cur.it.tile(cur.i) * TK;
+    const bool whole = cur.it.whole(p, k0);
+
+    float s[TK / 8][4];
+#pragma unroll
+    for (int n = 0; n < TK / 8; n += 2) {
+      float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        uint32_t b[4];  // keys 8n .. 8n+7 at features 0-7, 8-15, then keys 8n+8 .. 8n+15
+        ldmatrix_x4(sk + paged_rows_at<HD>(8 * n + (lane & 7) + (lane & 16 ? 8 : 0), 2 * kk + ((lane >> 3) & 1)), b);
+        PT::mma(s0, qf[kk], b[0], b[1]);
+        PT::mma(s1, qf[kk], b[2], b[3]);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[n][x] = s0[x] * p.scale_log2;
+        s[n + 1][x] = s1[x] * p.scale_log2;
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < TK / 8; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int key = k0 + 8 * n + lane % 4 * 2 + (x & 1), t = pos[x >> 1];
+          if (key > t || (p.window > 0 && t - key >= p.window && key >= p.sinks)) s[n][x] = -INFINITY;
+        }
+    }
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < TK / 8; ++n) {
+      top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
+      top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]));
+    }
+    float base[2];
+    bool moved = false;
+    float corr[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
+      const float next = fmaxf(m[h], top[h]);
+      base[h] = next == -INFINITY ? 0.f : next;  // a row that has seen no key: every 2^(s - 0) below is 0
+      corr[h] = ex2_approx(m[h] - base[h]);
+      moved |= next > m[h];
+      m[h] = next;
+      l[h] *= corr[h];
+    }
+    if (__any_sync(~0u, moved)) {
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d) {
+        o[d][0] *= corr[0];
+        o[d][1] *= corr[0];
+        o[d][2] *= corr[1];
+        o[d][3] *= corr[1];
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < TK / 8; n += 2) {
+      uint32_t pf[4];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float e0 = ex2_approx(s[n + g][0] - base[0]), e1 = ex2_approx(s[n + g][1] - base[0]);
+        const float e2 = ex2_approx(s[n + g][2] - base[1]), e3 = ex2_approx(s[n + g][3] - base[1]);
+        l[0] += e0 + e1;
+        l[1] += e2 + e3;
+        pf[2 * g] = PT::pack(e0, e1);
+        pf[2 * g + 1] = PT::pack(e2, e3);
+      }
+#pragma unroll
+      for (int d = 0; d < HD / 8; d += 2) {
+        uint32_t b[4];  // keys 8n .. 8n+15 (two halves) at features 8d .. 8d+7, then the next eight
+        ldmatrix_x4_trans(sv + paged_rows_at<HD>(8 * n + (lane & 15), d + (lane >> 4)), b);
+        PT::mma(o[d], pf, b[0], b[1]);
+        PT::mma(o[d + 1], pf, b[2], b[3]);
+      }
+    }
+    __syncwarp();  // every lane has read the stage before a later round refills it
+
+    const bool last = cur.i + 1 == cur.it.n;
+    if (last || u + 1 == n_units) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(~0u, l[h], 1);
+        l[h] += __shfl_xor_sync(~0u, l[h], 2);
+      }
+      if (last && from_start) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = lane / 4 + 8 * h;
+          if (row >= cur.it.rows) continue;
+          const float inv = l[h] > 0.f ? 1.f / l[h] : 0.f;
+          const int r = cur.it.r0 + row, tok = cur.s.q0 + r / p.group, head = cur.kvh * p.group + r % p.group;
+          T* dst = static_cast<T*>(p.out) + (static_cast<long long>(tok) * p.heads + head) * p.out_hd + lane % 4 * 2;
+#pragma unroll
+          for (int d = 0; d < HD / 8; ++d)
+            if (8 * d < p.out_hd)
+              *reinterpret_cast<uint32_t*>(dst + 8 * d) = PT::pack(o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
+        }
+      } else {
+        float* slot = p.part + (2ll * worker + (from_start ? 1 : 0)) * paged_slot_floats<16, HD>();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = lane / 4 + 8 * h;
+          if (row >= cur.it.rows) continue;
+          if (lane % 4 == 0) {
+            slot[16 * HD + row] = m[h];
+            slot[16 * HD + 16 + row] = l[h];
+          }
+#pragma unroll
+          for (int d = 0; d < HD / 8; ++d)
+            *reinterpret_cast<float2*>(slot + row * HD + 8 * d + lane % 4 * 2) =
+                make_float2(o[d][2 * h], o[d][2 * h + 1]);
+        }
+      }
+      fresh = true;
+      from_start = true;
+      if (u + 1 < n_units) cur.next_item(p, RPT);
+    } else {
+      ++cur.i;
+    }
+  }
+  cp_async_wait<0>();
+}
+
+}  // namespace tt

@@ -10,11 +10,12 @@ compose the ops themselves; the model path calls ``tt_model_forward`` once.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from ctypes import c_int64, c_size_t
+from typing import Dict, Optional, Tuple
 
 import torch
 
-from ._lib import check, lib
+from ._lib import KVCache, check, lib
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -175,3 +176,211 @@ def ffn_residual_layernorm(a: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, 
             resid_out.data_ptr(), norm.data_ptr(), n, D, w1.shape[0], float(eps),
             int(normalized_dtype == torch.float16), mask_ptr, _stream(a)))
     return resid_out, norm
+
+
+# ---------------------------------------------------------------------------
+# Paged K/V cache
+#
+# A cache is a few plain tensors: pages k, v [pages, kv_heads, page, hs] of one
+# layer (or [layers, pages, ...] where a call moves every layer), int32 tables
+# [slots, width] (-1: no page), lens [slots] and refs [pages].  A call's batch
+# entry b is slot slots[b] (slot b without ``slots``), and its new tokens are
+# rows cu_q[b] .. cu_q[b + 1] - 1 of the token tensors.  ``PagedKVCache`` keeps
+# these tensors together.
+# ---------------------------------------------------------------------------
+_PAGED_DTYPES = (torch.float16, torch.bfloat16)
+PAGE_SIZES = (16, 32, 64, 128, 256)
+
+
+def _index(t: Optional[torch.Tensor], name: str, device: torch.device, dims: int = 1) -> int:
+    """Address of an int32 index tensor (0 for None)."""
+    if t is None:
+        return 0
+    _need(t.dtype == torch.int32 and t.dim() == dims and t.device == device,
+          f"{name} must be an int32 tensor of {dims} dimension(s) on {device}")
+    _need(t.is_contiguous() if dims == 1 else t.stride(-1) == 1, f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _cache(k: Optional[torch.Tensor], v: Optional[torch.Tensor], tables: torch.Tensor, lens: torch.Tensor,
+           refs: Optional[torch.Tensor], page: int = 0) -> KVCache:
+    dev = tables.device
+    _need(tables.is_cuda, "tables must be a CUDA tensor")
+    c = KVCache()
+    c.tables, c.lens, c.refs = _index(tables, "tables", dev, 2), _index(lens, "lens", dev), _index(refs, "refs", dev)
+    c.n_slots, c.table_width = tables.shape
+    c.table_stride = tables.stride(0)
+    _need(lens.shape[0] == c.n_slots, f"lens has {lens.shape[0]} entries, tables {c.n_slots} rows")
+    if k is None:
+        c.page, c.n_pages = page, refs.shape[0]
+        return c
+    _need(k.dim() in (4, 5) and k.shape == v.shape, "k and v must be [pages, kv_heads, page, head_dim] pages of one "
+          "layer, or [layers, pages, ...], of one shape")
+    _need(k.dtype in _PAGED_DTYPES and v.dtype == k.dtype, "k and v pages must be FP16 or BF16")
+    _need(k.device == dev and v.device == dev, f"k and v pages must be on {dev}")
+    pages, c.kv_heads, c.page, c.head_dim = k.shape[-4:]
+    for t, name in ((k, "k"), (v, "v")):
+        st = t.stride()
+        _need(st[-1] == 1 and st[-2] == c.head_dim and st[-3] == c.page * c.head_dim,
+              f"each page of {name} must be contiguous")
+    c.k, c.v = k.data_ptr(), v.data_ptr()
+    c.k_page_stride, c.v_page_stride = k.stride(-4), v.stride(-4)
+    c.layers = 1
+    if k.dim() == 5:
+        c.layers, c.k_layer_stride, c.v_layer_stride = k.shape[0], k.stride(0), v.stride(0)
+    c.n_pages = pages
+    _need(refs is None or refs.shape[0] == pages, f"refs must have one entry for each of the {pages} pages")
+    return c
+
+
+def _run(device: torch.device, fn, *args) -> None:
+    """Calls a libtt_b200 entry point on the device's current stream."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, stream))
+        return
+    with torch.cuda.device(device):
+        check(fn(*args, stream))
+
+
+def _batch(cu_q: torch.Tensor, slots: Optional[torch.Tensor], tables: torch.Tensor) -> Tuple[int, int, int]:
+    """(address of cu_q, address of slots, sequences of the call)."""
+    n = cu_q.shape[0] - 1
+    _need(n >= 0, "cu_q needs at least one entry")
+    if slots is None:
+        _need(n <= tables.shape[0], f"{n} sequences, but {tables.shape[0]} table rows")
+    else:
+        _need(slots.shape[0] == n, f"cu_q describes {n} sequences, slots {slots.shape[0]}")
+    return _index(cu_q, "cu_q", tables.device), _index(slots, "slots", tables.device), n
+
+
+def cache_reserve(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, cu_q: torch.Tensor, page: int,
+                  slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Allocates the pages that the new tokens of (distinct) slots need and adds the tokens to ``lens``.
+
+    All or nothing.  Returns an int32 status [1] on the device: 0 done, > 0 that many pages are
+    missing, -1 a sequence would outgrow its table row, -2 a bad slot or cu_q.
+    """
+    c = _cache(None, None, tables, lens, refs, page)
+    cu, sl, n = _batch(cu_q, slots, tables)
+    status = torch.empty(1, dtype=torch.int32, device=tables.device)
+    _run(tables.device, lib().tt_cache_reserve, c, cu, sl, n, status.data_ptr())
+    return status
+
+
+def _token_strides(t: torch.Tensor):
+    return (c_int64 * 3)(*t.stride())
+
+
+def cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                 lens: torch.Tensor, cu_q: torch.Tensor, slots: Optional[torch.Tensor] = None) -> None:
+    """Writes the new tokens' k, v [tokens, kv_heads, hs] into one layer's pages; ``lens`` counts them already.
+
+    k and v may be strided views that are dense in their features, or dense in their tokens
+    (``qkv_projection``'s vt as ``vt[0, :, :, :n].permute(2, 0, 1)``).
+    """
+    c = _cache(k_pages, v_pages, tables, lens, None)
+    want = (k.shape[0], c.kv_heads, c.head_dim)
+    _need(k_pages.dim() == 4, "append writes one layer's pages")
+    _need(tuple(k.shape) == want and tuple(v.shape) == want, f"k and v must be [tokens, {want[1]}, {want[2]}]")
+    _need(k.dtype == k_pages.dtype and v.dtype == k_pages.dtype, "k and v must have the pages' dtype")
+    _need(k.device == tables.device and v.device == tables.device, f"k and v must be on {tables.device}")
+    cu, sl, n = _batch(cu_q, slots, tables)
+    _run(tables.device, lib().tt_cache_append, c, k.data_ptr(), _token_strides(k), v.data_ptr(), _token_strides(v),
+         want[0], cu, sl, n)
+
+
+def cache_release(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, page: int,
+                  slots: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0) -> None:
+    """Frees the slots (all without ``slots``), or with a window the pages that no later query of them can see."""
+    c = _cache(None, None, tables, lens, refs, page)
+    n = tables.shape[0] if slots is None else slots.shape[0]
+    _run(tables.device, lib().tt_cache_release, c, _index(slots, "slots", tables.device), n, int(window), int(sinks))
+
+
+def cache_fork(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
+               refs: torch.Tensor, parents: torch.Tensor, children: torch.Tensor) -> torch.Tensor:
+    """Makes each (empty, distinct) child slot a copy of its parent: full pages are shared, a partial one is copied.
+
+    All or nothing.  Returns an int32 status [1]: 0 done, > 0 pages missing, -1 a parent without
+    its last page, -2 a bad slot, -3 a child that is not empty or occurs twice.
+    """
+    c = _cache(k_pages, v_pages, tables, lens, refs)
+    dev = tables.device
+    _need(parents.shape == children.shape, "parents and children must have one length")
+    n = parents.shape[0]
+    buf = torch.empty(2 * n + 2, dtype=torch.int32, device=dev)
+    status = buf[:1]
+    _run(dev, lib().tt_cache_fork, c, _index(parents, "parents", dev), _index(children, "children", dev), n,
+         buf.data_ptr() + 4, status.data_ptr())
+    return status
+
+
+def cache_compact(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
+                  refs: torch.Tensor) -> torch.Tensor:
+    """Moves the live pages to the front of the pool, tables and refs with them; returns their number, int32 [1]."""
+    c = _cache(k_pages, v_pages, tables, lens, refs)
+    buf = torch.empty(3 * c.n_pages + 3, dtype=torch.int32, device=tables.device)
+    live = buf[:1]
+    _run(tables.device, lib().tt_cache_compact, c, buf.data_ptr() + 4, live.data_ptr())
+    return live
+
+
+def cache_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
+                     src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copies pages src[i] -> dst[i] of every layer (no destination twice, none of them a source)."""
+    c = _cache(k_pages, v_pages, tables, lens, None)
+    dev = tables.device
+    _need(src.shape == dst.shape, "src and dst must have one length")
+    _run(dev, lib().tt_cache_copy_pages, c, _index(src, "src", dev), _index(dst, "dst", dev), src.shape[0])
+
+
+_paged_ws_bytes: Dict[tuple, int] = {}
+
+
+def _paged_workspace(device: torch.device, heads: int, kv_heads: int, head_dim: int, max_q_len: int) -> torch.Tensor:
+    key = (device.index, heads, kv_heads, head_dim, max_q_len)
+    need = _paged_ws_bytes.get(key)
+    if need is None:
+        nbytes = c_size_t()
+        with torch.cuda.device(device):
+            check(lib().tt_paged_attention_workspace_bytes(heads, kv_heads, head_dim, max_q_len, nbytes))
+        need = _paged_ws_bytes[key] = int(nbytes.value)
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                    lens: torch.Tensor, cu_q: torch.Tensor, *, slots: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None, window: int = 0, sinks: int = 0, head_dim: Optional[int] = None,
+                    max_q_len: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of new tokens over one layer's pages -> [tokens, heads * hd] in the pages' dtype.
+
+    q [tokens, heads, hs] (dense features, any token and head strides of whole 16 bytes); heads a
+    multiple of the pages' kv_heads.  The T new tokens of a sequence are its last T positions
+    (``lens`` counts them).  With ``window`` a query sees the last ``window`` keys, itself included,
+    and the first ``sinks`` ones.  A row that sees no key, or belongs to no sequence, is zero.
+    ``head_dim`` 8 takes pages stored 16 wide; ``max_q_len``, if known, bounds every T.
+    """
+    c = _cache(k_pages, v_pages, tables, lens, None)
+    dev = tables.device
+    _need(k_pages.dim() == 4, "attention reads one layer's pages")
+    _need(q.dim() == 3 and q.shape[2] == c.head_dim, f"q must be [tokens, heads, {c.head_dim}]")
+    _need(q.dtype == k_pages.dtype and q.device == dev, "q must have the pages' dtype and device")
+    n, heads, hs = q.shape
+    st = q.stride()
+    _need(st[2] == 1 or n == 0, "q must be dense in its features")
+    _need(heads % c.kv_heads == 0, f"{heads} query heads are not a multiple of {c.kv_heads} KV heads")
+    hd = hs if head_dim is None else int(head_dim)
+    _need(window >= 0 and sinks >= 0, "window and sinks must not be negative")
+    cu, sl, batch = _batch(cu_q, slots, tables)
+    if out is None:
+        out = torch.empty(n, heads * hd, dtype=q.dtype, device=dev)
+    else:
+        _need(out.shape == (n, heads * hd) and out.dtype == q.dtype and out.device == dev and out.is_contiguous(),
+              f"out must be a contiguous [{n}, {heads * hd}] tensor of q's dtype on {dev}")
+    bound = n if max_q_len is None else int(max_q_len)
+    ws = _paged_workspace(dev, heads, c.kv_heads, hd, 0)
+    _run(dev, lib().tt_paged_attention, c, q.data_ptr(), st[0], st[1], cu, sl, batch, out.data_ptr(), n, heads, hd,
+         q.dtype is torch.bfloat16, hd ** -0.5 if scale is None else float(scale), window, sinks, bound, ws.data_ptr(),
+         ws.numel())
+    return out
