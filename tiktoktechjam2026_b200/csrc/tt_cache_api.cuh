@@ -6,6 +6,7 @@
 
 #include "tt_cache.cuh"
 #include "tt_paged_attn.cuh"
+#include "tt_paged_chunk.cuh"
 
 namespace {
 
@@ -69,13 +70,18 @@ int cache_params(const tt_kv_cache* c, bool values, bool counts, CacheParams* ou
 }
 
 // ---------------------------------------------------------------- attention
+// Sequences of at most this many query rows (tokens * group) take the kernel
+// for short chunks, whose items hold that many rows.
+constexpr int kRowsMax = 16;
 // Units that a worker takes at least: fewer would cost more in joining than
 // the shorter pieces save.
-constexpr long long kRowsMinUnits = 2;
+constexpr long long kRowsMinUnits = 2, kChunkMinUnits = 4;
 
 template <int HD>
 size_t paged_part_bytes(int sm_count) {
-  return 2ull * sm_count * PagedRowsLayout<HD>::WARPS * paged_slot_floats<16, HD>() * sizeof(float);
+  const size_t rows = 2ull * sm_count * PagedRowsLayout<HD>::WARPS * paged_slot_floats<kRowsMax, HD>();
+  const size_t chunk = 2ull * sm_count * paged_slot_floats<PagedChunkLayout<HD>::ROWS, HD>();
+  return (rows > chunk ? rows : chunk) * sizeof(float);
 }
 
 int paged_workspace(int hd, int sm_count, size_t* bytes) {
@@ -90,19 +96,63 @@ int paged_workspace(int hd, int sm_count, size_t* bytes) {
   }
 }
 
+// Sequences of row_lo .. row_hi query rows.
 template <typename T, int HD>
-int launch_paged(PagedParams p, int max_rows, int sm_count, cudaStream_t stream) {
+int launch_paged_rows(PagedParams p, int row_lo, int row_hi, int sm_count, cudaStream_t stream) {
   using L = PagedRowsLayout<HD>;
-  (void)max_rows;
   auto kern = paged_rows_kernel<T, HD>;
   if (int rc = prepare_kernel(kern, L::SMEM)) return rc;
-  p.row_lo = 0;
-  p.row_hi = 0x7fffffff;
+  p.row_lo = row_lo;
+  p.row_hi = row_hi;
   p.n_workers = sm_count * L::WARPS;
   launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, p, kRowsMinUnits);
-  if (int rc = after_launch("paged attention")) return rc;
-  launch_kernel(paged_join_kernel<T, HD, L::TK, 16, 16, 256>, p.n_workers - 1, 256, 0, stream, p, 16, kRowsMinUnits);
+  if (int rc = after_launch("paged attention (rows)")) return rc;
+  launch_kernel(paged_join_kernel<T, HD, L::TK, kRowsMax, kRowsMax, 256>, p.n_workers - 1, 256, 0, stream, p, kRowsMax,
+                kRowsMinUnits);
   return after_launch("paged attention join");
+}
+
+template <typename T, int HD>
+int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t stream) {
+  using L = PagedChunkLayout<HD>;
+  auto kern = paged_chunk_kernel<T, HD>;
+  KernelInfo ki;
+  if (int rc = kernel_info(reinterpret_cast<const void*>(kern), L::SMEM, &ki)) return rc;
+  if (L::SPLIT ? ki.regs != L::REGS_LAUNCH : ki.regs > 255)
+    return fail(TT_ERR_UNSUPPORTED, "paged attention kernel built with %d registers per thread, expected %d", ki.regs,
+                L::REGS_LAUNCH);
+  p.row_lo = row_lo;
+  p.row_hi = 0x7fffffff;
+  p.n_workers = sm_count;
+  const int half_tokens = 128 / p.group, page = 1 << p.page_shift;
+  CUtensorMap tq, tk, tv;
+  {
+    const uint64_t dims[3] = {HD, static_cast<uint64_t>(p.heads), static_cast<uint64_t>(p.n_tokens)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(p.q_head) * 2, static_cast<uint64_t>(p.q_token) * 2};
+    const uint32_t box[3] = {L::ATOM, static_cast<uint32_t>(p.group), static_cast<uint32_t>(half_tokens)};
+    if (int rc = encode_f16(&tq, p.q, 3, dims, strides, box)) return rc;
+  }
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint64_t dims[3] = {HD, static_cast<uint64_t>(p.kv_heads) * page, static_cast<uint64_t>(p.n_pages)};
+    const uint64_t strides[2] = {HD * 2, static_cast<uint64_t>(kv ? p.v_stride : p.k_stride) * 2};
+    const uint32_t box[3] = {L::ATOM, static_cast<uint32_t>(page < L::BN ? page : L::BN), 1};
+    if (int rc = encode_f16(kv ? &tv : &tk, kv ? p.v_pages : p.k_pages, 3, dims, strides, box)) return rc;
+  }
+  launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, tq, tk, tv, p, half_tokens, kChunkMinUnits);
+  if (int rc = after_launch("paged attention (chunk)")) return rc;
+  constexpr int RB = 32;
+  launch_kernel(paged_join_kernel<T, HD, L::BN, L::ROWS, RB, 256>, dim3(sm_count - 1, L::ROWS / RB), 256, 0, stream, p,
+                L::NT * half_tokens * p.group, kChunkMinUnits);
+  return after_launch("paged attention join");
+}
+
+// Each sequence goes by its own number of query rows; max_rows only saves
+// launches whose kernel could have no work.
+template <typename T, int HD>
+int launch_paged(const PagedParams& p, int max_rows, int sm_count, cudaStream_t stream) {
+  if (max_rows <= kRowsMax) return launch_paged_rows<T, HD>(p, 0, 0x7fffffff, sm_count, stream);
+  if (int rc = launch_paged_chunk<T, HD>(p, kRowsMax + 1, sm_count, stream)) return rc;
+  return launch_paged_rows<T, HD>(p, 0, kRowsMax, sm_count, stream);
 }
 
 template <typename T>
