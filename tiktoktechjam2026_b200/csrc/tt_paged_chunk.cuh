@@ -34,10 +34,9 @@ template <int HD>
 struct PagedChunkLayout {
   static constexpr int NT = HD == 256 ? 1 : 2;      // halves
   static constexpr int ROWS = 128 * NT;             // rows of a workspace slot
-  static constexpr int BN = HD == 128 ? 128 : 64;   // keys per tile
-  static constexpr int NSB = HD == 128 ? 1 : 3;     // S buffers per half
-  static constexpr int NSK = HD == 128 ? 3 : HD == 256 ? 2 : 6;  // K and V tiles in the ring
-  static constexpr int NSV = HD == 128 ? 2 : HD == 256 ? 2 : 6;
+  static constexpr int BN = 64;                     // keys per tile
+  static constexpr int NSB = HD >= 128 ? 2 : 3;      // S buffers per half
+  static constexpr int NST = HD == 256 ? 2 : HD == 128 ? 5 : 8;   // stages of a K and a V tile
   static constexpr int NQ = HD >= 128 ? 1 : 2;      // Q tile buffers per half
   static constexpr int NOB = HD <= 32 ? 2 : 1;      // O buffers per half
   static constexpr int ATOM = HD >= 64 ? 64 : HD;   // features per swizzle atom
@@ -47,13 +46,13 @@ struct PagedChunkLayout {
   static constexpr int Q_BYTES = NATOM * Q_ATOM, KV_BYTES = NATOM * KV_ATOM;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = NT * NQ * Q_BYTES;
-  static constexpr int OFF_V = OFF_K + NSK * KV_BYTES;
-  static constexpr int OFF_BAR = OFF_V + NSV * KV_BYTES;
-  // Barriers: K full/empty, V full/empty/fixed, then per half Q full/empty,
-  // S full, P full, PV done, O full/free, done.
-  static constexpr int B_KF = 0, B_KE = NSK, B_VF = 2 * NSK, B_VE = B_VF + NSV, B_VX = B_VE + NSV, B_HALF = B_VX + NSV;
-  static constexpr int H_QF = 0, H_QE = 2, H_SF = 4, H_PF = H_SF + NSB, H_PE = H_PF + NSB, H_OF = H_PE + NSB,
-                       H_OR = H_OF + 2, H_DONE = H_OR + 2, N_HALF = H_DONE + 1;
+  static constexpr int OFF_V = OFF_K + NST * KV_BYTES;
+  static constexpr int OFF_BAR = OFF_V + NST * KV_BYTES;
+  // Barriers: stage full / empty / stale rows zeroed, then per half Q
+  // full / empty, S full, P full, O full / free, done.
+  static constexpr int B_F = 0, B_E = NST, B_X = 2 * NST, B_HALF = 3 * NST;
+  static constexpr int H_QF = 0, H_QE = 2, H_SF = 4, H_PF = H_SF + NSB, H_OF = H_PF + NSB, H_OR = H_OF + 2,
+                       H_DONE = H_OR + 2, N_HALF = H_DONE + 1;
   static constexpr int OFF_MISC = OFF_BAR + (B_HALF + NT * N_HALF) * 8;
   static constexpr int SMEM = OFF_MISC + 16 + 1024;
   static constexpr int TMEM_COLS = 512, TMEM_O = NSB * BN, TMEM_HALF = 512 / NT;
@@ -66,9 +65,11 @@ struct PagedChunkLayout {
   // warps carry two walks of the piece, the softmax warps a row of BN scores.
   static constexpr bool SPLIT = NT == 2;
   static constexpr int REGS_LAUNCH = 168;
-  static constexpr int REGS_SOFTMAX = BN == 128 ? 208 : 184, REGS_OTHER = BN == 128 ? 88 : 136;
+  static constexpr int REGS_SOFTMAX = 184, REGS_OTHER = 136;
   static_assert(!SPLIT || 128 * NT * REGS_SOFTMAX + 32 * (NWARPS - 4 * NT) * REGS_OTHER <= THREADS * REGS_LAUNCH,
                 "register split");
+  // A stage is waited for while the NSB before it but one are held.
+  static_assert(NST >= NSB, "ring depth");
   static_assert(TMEM_O + NOB * HD <= TMEM_HALF, "TMEM budget");
   static_assert(SMEM <= 232448, "shared memory budget");
   static_assert(Q_BYTES % 1024 == 0 && KV_BYTES % 1024 == 0 && OFF_BAR % 1024 == 0, "alignment");
@@ -111,6 +112,17 @@ __device__ __forceinline__ uint64_t exp2_pair_wide(uint64_t yy) {
   return (static_cast<uint64_t>(r1) << 32) | r0;
 }
 
+// True in one lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ uint32_t bits_below(int x) {  // the lowest x bits (none below 0, all from 32)
   return x >= 32 ? ~0u : (x <= 0 ? 0u : (1u << x) - 1u);
 }
@@ -129,54 +141,66 @@ struct ChunkRange {
   }
 };
 
-// Walks a worker's piece segment by segment (a segment is the part of one item
-// that lies in the piece) for one half.
+// One half of a segment (a segment is the part of one item that lies in the piece).
+struct ChunkHalf {
+  int rows;        // query rows
+  int p0, p1;      // positions of the first and last row
+  ChunkRange range;
+  int last;        // the last tile of the segment that it sees, -1: none
+};
+
+// Walks a worker's piece segment by segment.
 template <int HD>
 struct ChunkWalk {
   using L = PagedChunkLayout<HD>;
   static constexpr int BN = L::BN;
   PagedCursor<BN> cur;
-  int left;        // units of the piece from this segment on
-  int i0, i1;      // the segment's tiles
-  int rows;        // rows of this half
-  int p0, p1;      // positions of its first and last row
-  ChunkRange range;
-  int last;        // its last tile in the segment, -1: none
-  __device__ __forceinline__ void load(const PagedParams& p, int half, int half_tokens) {
-    const int hr = half_tokens * p.group;
+  int left;    // units of the piece from this segment on
+  int i0, i1;  // the segment's tiles
+  __device__ __forceinline__ void load() {
     i0 = cur.i;
     i1 = min(cur.it.n, i0 + left);
-    rows = min(max(cur.it.rows - half * hr, 0), hr);
-    range = {0, 0, 0};
-    last = -1;
-    if (rows == 0) return;
-    p0 = cur.it.p0 + half * half_tokens;
-    p1 = cur.it.p0 + half * half_tokens + (rows - 1) / p.group;
-    const int end = p1 < 0 ? 0 : p1 / BN + 1;  // one past the last tile a row sees
-    if (p.window == 0) {
-      range.e = end;
-    } else {
-      const int from = max(p0 - p.window + 1, 0) / BN;  // first tile in the window
-      const int sink = (min(p.sinks, BN * end) + BN - 1) / BN;
-      if (cur.it.n_sink == cur.it.n) {  // no gap: the index is the tile
-        range.a = min(sink, end);
-        range.c = max(from, range.a);
-        range.e = end;
-      } else {
-        range.a = min(cur.it.n_sink, end);
-        range.c = max(from - cur.it.w_tile, 0) + cur.it.n_sink;
-        range.e = end - cur.it.w_tile + cur.it.n_sink;
-      }
-    }
-    last = range.last(i0, i1);
+  }
+  __device__ __forceinline__ void begin(const PagedParams& p, const PagedStart& s, int n_units, int rpt) {
+    cur.seek(p, s.b, s.off, rpt);
+    left = n_units;
+    load();
   }
   // The next segment; false at the end of the piece.
-  __device__ __forceinline__ bool next(const PagedParams& p, int half, int half_tokens, int rpt) {
+  __device__ __forceinline__ bool next(const PagedParams& p, int rpt) {
     left -= i1 - i0;
     if (left <= 0) return false;
     cur.next_item(p, rpt);
-    load(p, half, half_tokens);
+    load();
     return true;
+  }
+  __device__ __forceinline__ ChunkHalf half(const PagedParams& p, int h, int half_tokens) const {
+    ChunkHalf x;
+    const int hr = half_tokens * p.group;
+    x.rows = min(max(cur.it.rows - h * hr, 0), hr);
+    x.range = {0, 0, 0};
+    x.last = -1;
+    x.p0 = cur.it.p0 + h * half_tokens;
+    x.p1 = x.p0 + (x.rows - 1) / p.group;
+    if (x.rows == 0) return x;
+    const int end = x.p1 < 0 ? 0 : x.p1 / BN + 1;  // one past the last tile a row sees
+    if (p.window == 0) {
+      x.range.e = end;
+    } else {
+      const int from = max(x.p0 - p.window + 1, 0) / BN;  // first tile in the window
+      const int sink = (min(p.sinks, BN * end) + BN - 1) / BN;
+      if (cur.it.n_sink == cur.it.n) {  // no gap: the index is the tile
+        x.range.a = min(sink, end);
+        x.range.c = max(from, x.range.a);
+        x.range.e = end;
+      } else {
+        x.range.a = min(cur.it.n_sink, end);
+        x.range.c = max(from - cur.it.w_tile, 0) + cur.it.n_sink;
+        x.range.e = end - cur.it.w_tile + cur.it.n_sink;
+      }
+    }
+    x.last = x.range.last(i0, i1);
+    return x;
   }
 };
 
@@ -191,9 +215,10 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
                        long long min_units) {
   using L = PagedChunkLayout<HD>;
   using PT = Pair16<T>;
-  constexpr int BN = L::BN, NT = L::NT, NSB = L::NSB, NSK = L::NSK, NSV = L::NSV, NQ = L::NQ, NOB = L::NOB;
+  constexpr int BN = L::BN, NT = L::NT, NSB = L::NSB, NST = L::NST, NQ = L::NQ, NOB = L::NOB;
   extern __shared__ uint8_t smem_raw[];
   __shared__ PagedStart start;
+  __shared__ ChunkWalk<HD> saved[6 * NT];  // walks at rest: the softmax warps', then two of each MMA warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half_rows = half_tokens * p.group, rpt = NT * half_rows;
   long long total, per;
@@ -207,14 +232,10 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NSK; ++i) {
-      mbar_init(&bars[L::B_KF + i], 1);
-      mbar_init(&bars[L::B_KE + i], NT);
-    }
-    for (int i = 0; i < NSV; ++i) {
-      mbar_init(&bars[L::B_VF + i], 1);
-      mbar_init(&bars[L::B_VE + i], NT + 1);  // the MMA warps and the warp that zeroes stale rows
-      mbar_init(&bars[L::B_VX + i], 1);
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(&bars[L::B_F + i], 1);
+      mbar_init(&bars[L::B_E + i], NT + 1);  // the MMA warps and the warp that zeroes stale rows
+      mbar_init(&bars[L::B_X + i], 1);
     }
     for (int h = 0; h < NT; ++h) {
       uint64_t* b = bars + L::B_HALF + h * L::N_HALF;
@@ -227,7 +248,6 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
       for (int i = 0; i < NSB; ++i) {
         mbar_init(&b[L::H_SF + i], 1);
         mbar_init(&b[L::H_PF + i], 4);
-        mbar_init(&b[L::H_PE + i], 1);
       }
       mbar_init(&b[L::H_DONE], 1);
     }
@@ -256,16 +276,14 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
       tma_prefetch_desc(&tmV);
     }
     const int box = min(page_rows, BN), n_box = BN / box;  // boxes of a tile: lane i fetches the i-th
-    int u = 0, nq[NT] = {};
+    int u = 0, st = 0, nq[NT] = {};
+    uint32_t ph = 0;
     bool ok = true;
-    walk.cur.seek(p, start.b, start.off, rpt);
-    walk.left = n_units;
-    walk.load(p, 0, half_tokens);
+    walk.begin(p, start, n_units, rpt);
     do {
 #pragma unroll
       for (int h = 0; h < NT; ++h) {
-        walk.load(p, h, half_tokens);
-        if (walk.last < 0) continue;
+        if (walk.half(p, h, half_tokens).last < 0) continue;
         uint64_t* b = bars + L::B_HALF + h * L::N_HALF;
         const int qb = nq[h] % NQ;
         if (lane == 0) ok = wait_phase(&b[L::H_QE + qb], ((nq[h] / NQ) & 1) ^ 1, wd, 0x531);
@@ -294,162 +312,205 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
       for (int i = walk.i0; i < walk.i1; ++i, ++u) {
         const int next = i + 1 < walk.i1 ? page_of(i + 1) : 0;  // a tile ahead: its latency is off the path
         const int at = walk.cur.kvh * page_rows + ((walk.cur.it.tile(i) * BN + lane * box) & (page_rows - 1));
+        if (lane == 0) {
+          ok = wait_phase(&bars[L::B_E + st], ph ^ 1, wd, 0x532);
+          if (ok) mbar_arrive_expect_tx(&bars[L::B_F + st], 2 * L::KV_BYTES);
+        }
+        if (!(ok = __shfl_sync(~0u, ok, 0))) break;
+        if (lane < n_box) {
+          uint8_t* dst = smem + L::OFF_K + st * L::KV_BYTES + lane * box * L::ROW;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int st = u % (kv ? NSV : NSK), ph = u / (kv ? NSV : NSK);
-          uint64_t* full = &bars[(kv ? L::B_VF : L::B_KF) + st];
-          if (lane == 0) {
-            ok = wait_phase(&bars[(kv ? L::B_VE : L::B_KE) + st], (ph & 1) ^ 1, wd, 0x532 + kv);
-            if (ok) mbar_arrive_expect_tx(full, L::KV_BYTES);
+          for (int a = 0; a < L::NATOM; ++a) {
+            tma_load_3d(dst + a * L::KV_ATOM, &tmK, &bars[L::B_F + st], a * L::ATOM, at, page);
+            tma_load_3d(dst + NST * L::KV_BYTES + a * L::KV_ATOM, &tmV, &bars[L::B_F + st], a * L::ATOM, at, page);
           }
-          if (!(ok = __shfl_sync(~0u, ok, 0))) break;
-          if (lane < n_box) {
-            uint8_t* dst = smem + (kv ? L::OFF_V : L::OFF_K) + st * L::KV_BYTES + lane * box * L::ROW;
-#pragma unroll
-            for (int a = 0; a < L::NATOM; ++a)
-              tma_load_3d(dst + a * L::KV_ATOM, kv ? &tmV : &tmK, full, a * L::ATOM, at, page);
-          }
-          __syncwarp();
+        }
+        __syncwarp();
+        if (++st == NST) {
+          st = 0;
+          ph ^= 1;
         }
         if (!ok) break;
         page = next;
       }
-    } while (ok && walk.next(p, 0, half_tokens, rpt));
+    } while (ok && walk.next(p, rpt));
     // Let every copy this warp started land before the CTA may exit.
     if (lane == 0) {
       for (int h = 0; h < NT; ++h)
         for (int i = max(nq[h] - NQ, 0); i < nq[h]; ++i)
           wait_drain(&bars[L::B_HALF + h * L::N_HALF + L::H_QF + i % NQ], (i / NQ) & 1, kDrainLimitNs);
-      for (int i = max(u - NSK, 0); i < u; ++i) wait_drain(&bars[L::B_KF + i % NSK], (i / NSK) & 1, kDrainLimitNs);
-      for (int i = max(u - NSV, 0); i < u; ++i) wait_drain(&bars[L::B_VF + i % NSV], (i / NSV) & 1, kDrainLimitNs);
+      for (int i = max(u - NST, 0); i < u; ++i) wait_drain(&bars[L::B_F + i % NST], (i / NST) & 1, kDrainLimitNs);
     }
   } else if (warp == L::W_FIX) {
     // -------------------------------------------------------------- zeroes the stale rows of V
     if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_OTHER));
-    int u = 0;
+    int st = 0;
+    uint32_t ph = 0;
     bool ok = true;
-    walk.cur.seek(p, start.b, start.off, rpt);
-    walk.left = n_units;
-    walk.load(p, 0, half_tokens);
+    walk.begin(p, start, n_units, rpt);
     do {
-      const int n_keys = walk.cur.s.L;
-      for (int i = walk.i0; i < walk.i1; ++i, ++u) {
-        const int st = u % NSV, k0 = walk.cur.it.tile(i) * BN;
-        if (!(ok = warp_wait_phase(&bars[L::B_VF + st], (u / NSV) & 1, wd, 0x534))) break;
-        const int r0 = n_keys - k0;
-        const int r1 = ((r0 + page_rows - 1) & ~(page_rows - 1));  // k0 or the tile is a whole number of pages
-        if (r0 > 0 && r0 < BN && r1 > r0) {
+      // Only the item's last tile can hold the end of the sequence.
+      const int r0 = walk.cur.s.L - walk.cur.it.tile(walk.cur.it.n - 1) * BN;
+      const int r1 = min((r0 + page_rows - 1) & ~(page_rows - 1), BN);  // the end of its page, or of the tile
+      const int fix_at = r0 > 0 && r0 < BN && (r0 & (page_rows - 1)) != 0 ? walk.cur.it.n - 1 : -1;
+      for (int i = walk.i0; i < walk.i1; ++i) {
+        if (!(ok = warp_wait_phase(&bars[L::B_F + st], ph, wd, 0x534))) break;
+        if (i == fix_at) {
           const uint32_t base = smem_u32(smem + L::OFF_V + st * L::KV_BYTES);
           for (int a = 0; a < L::NATOM; ++a)
-            for (int x = r0 * L::ROW + lane * 16; x < min(r1, BN) * L::ROW; x += 512)
+            for (int x = r0 * L::ROW + lane * 16; x < r1 * L::ROW; x += 512)
               st_shared_v4(base + a * L::KV_ATOM + x, 0, 0, 0, 0);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[L::B_VX + st]);
+          if (lane == 0) mbar_arrive(&bars[L::B_X + st]);
         }
-        if (lane == 0) mbar_arrive(&bars[L::B_VE + st]);
+        if (lane == 0) mbar_arrive(&bars[L::B_E + st]);
+        if (++st == NST) {
+          st = 0;
+          ph ^= 1;
+        }
       }
-    } while (ok && walk.next(p, 0, half_tokens, rpt));
+    } while (ok && walk.next(p, rpt));
   } else if (warp >= L::W_MMA && warp < L::W_MMA + NT) {
     // -------------------------------------------------------------- MMA issuer of a half
+    // The warp's own instructions are on the critical path.  It walks the loop
+    // as a whole on values that shuffles and votes make warp-uniform, and one
+    // elected lane issues: in a region of a single lane every operand would go
+    // through vector registers.
     if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_OTHER));
+    const int h = __shfl_sync(~0u, warp - L::W_MMA, 0);
+    uint64_t* b = bars + L::B_HALF + h * L::N_HALF;
+    const uint32_t sbase = smem_u32(smem);
+    constexpr uint32_t kSw = swizzle_kind_for_bytes(L::ROW), kSbo = 8 * L::ROW;
+    constexpr uint32_t idesc_s = umma_idesc_16(128, BN, PT::kBf16, false);
+    constexpr uint32_t idesc_o = umma_idesc_16(128, HD, PT::kBf16, true);
+    const uint64_t dq0 = umma_sdesc(sbase + L::OFF_Q + h * NQ * L::Q_BYTES, kSbo, kSw);
+    const uint64_t dk0 = umma_sdesc(sbase + L::OFF_K, kSbo, kSw);
+    const uint64_t dv0 = umma_sdesc_mn(sbase + L::OFF_V, L::KV_ATOM, kSbo, kSw);
+    const uint32_t tS = __shfl_sync(~0u, tmem_base, 0) + h * L::TMEM_HALF;
+    // Two walks of the piece, in shared memory: [0] for the scores, which run
+    // NSB units ahead (counted in units and not in the half's tiles: the producer
+    // can then always fill what is waited for), [1] for P.V.
+    ChunkWalk<HD>* walks = saved + 4 * NT + 2 * h;
+    struct Segment {  // warp-uniform
+      int i, i1, a, c, e, last, fix_at;
+      __device__ __forceinline__ bool has() const { return i < a || (i >= c && i < e); }
+    };
+    auto read = [&](const ChunkWalk<HD>& w) -> Segment {
+      const ChunkHalf x = w.half(p, h, half_tokens);
+      const int r0 = w.cur.s.L - w.cur.it.tile(w.cur.it.n - 1) * BN;
+      const int fix = r0 > 0 && r0 < BN && (r0 & (page_rows - 1)) != 0 ? w.cur.it.n - 1 : -1;
+      return {__shfl_sync(~0u, w.i0, 0),      __shfl_sync(~0u, w.i1, 0),      __shfl_sync(~0u, x.range.a, 0),
+              __shfl_sync(~0u, x.range.c, 0), __shfl_sync(~0u, x.range.e, 0), __shfl_sync(~0u, x.last, 0),
+              __shfl_sync(~0u, fix, 0)};
+    };
     if (lane == 0) {
-      const int h = warp - L::W_MMA;
-      uint64_t* b = bars + L::B_HALF + h * L::N_HALF;
-      const uint32_t sbase = smem_u32(smem);
-      const uint32_t tS = tmem_base + h * L::TMEM_HALF;
-      constexpr uint32_t kSw = swizzle_kind_for_bytes(L::ROW), kSbo = 8 * L::ROW;
-      constexpr uint32_t idesc_s = umma_idesc_16(128, BN, PT::kBf16, false);
-      constexpr uint32_t idesc_o = umma_idesc_16(128, HD, PT::kBf16, true);
-      bool ok = true;
-      // Score cursor: segment walk, tile i, ring position us, this half's tile t_s and segment count q_s.
-      walk.cur.seek(p, start.b, start.off, rpt);
-      walk.left = n_units;
-      walk.load(p, h, half_tokens);
-      ChunkWalk<HD> pv = walk;
-      int i_s = walk.i0, us = 0, t_s = 0, q_s = 0;
-      bool more_s = true, q_ready = false;
-      // Scores of the next unit; a tile that this half does not see is handed
-      // back.  It runs NSB units ahead of P.V, counted in units and not in this
-      // half's tiles: the producer may then always fill what is waited for.
-      auto step_s = [&]() -> bool {
-        while (more_s && i_s == walk.i1) {
-          q_ready = false;
-          more_s = walk.next(p, h, half_tokens, rpt);
-          i_s = walk.i0;
-        }
+      walks[0].begin(p, start, n_units, rpt);
+      walks[1] = walks[0];
+    }
+    __syncwarp();
+    Segment ss = read(walks[0]);
+    int k_st = 0, s_buf = 0, q_buf = 0;
+    uint32_t k_ph = 0, q_ph = 0;
+    bool more_s = true, q_new = true;
+    // Waits for the next unit's stage and issues its scores, if this half sees it.
+    auto step_s = [&]() -> bool {
+      if (ss.i == ss.i1) {
         if (!more_s) return true;
-        const int st = us % NSK;
-        const bool mine = walk.range.has(i_s);
-        if (mine && !q_ready) {
-          if (!wait_phase(&b[L::H_QF + q_s % NQ], (q_s / NQ) & 1, wd, 0x535)) return false;
-          q_ready = true;
+        more_s = __shfl_sync(~0u, lane == 0 ? walks[0].next(p, rpt) : false, 0);
+        __syncwarp();
+        if (!more_s) return true;
+        ss = read(walks[0]);
+        q_new = true;
+      }
+      if (!warp_wait_phase(&bars[L::B_F + k_st], k_ph, wd, 0x536)) return false;
+      if (ss.has()) {
+        if (q_new) {
+          if (!warp_wait_phase(&b[L::H_QF + q_buf], q_ph, wd, 0x535)) return false;
+          q_new = false;
         }
-        if (!wait_phase(&bars[L::B_KF + st], (us / NSK) & 1, wd, 0x536)) return false;
-        ++us;
-        if (mine) {
-          tc_fence_after();
-          const uint32_t sq = sbase + L::OFF_Q + (h * NQ + q_s % NQ) * L::Q_BYTES;
-          const uint32_t sk = sbase + L::OFF_K + st * L::KV_BYTES;
+        tc_fence_after();
+        const uint64_t dq = dq0 + (q_buf * L::Q_BYTES >> 4), dk = dk0 + (k_st * L::KV_BYTES >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const int at = 16 * kk / L::ATOM, off = 16 * kk % L::ATOM * 2;
-            umma_f16(tS + t_s % NSB * BN, umma_sdesc(sq + at * L::Q_ATOM + off, kSbo, kSw),
-                     umma_sdesc(sk + at * L::KV_ATOM + off, kSbo, kSw), idesc_s, kk > 0 ? 1u : 0u);
+            umma_f16(tS + s_buf * BN, dq + ((at * L::Q_ATOM + off) >> 4), dk + ((at * L::KV_ATOM + off) >> 4), idesc_s,
+                     kk > 0 ? 1u : 0u);
           }
-          umma_commit(&b[L::H_SF + t_s % NSB]);
-          umma_commit(&bars[L::B_KE + st]);
-          if (i_s == walk.last) umma_commit(&b[L::H_QE + q_s++ % NQ]);
-          ++t_s;
-        } else {
-          mbar_arrive(&bars[L::B_KE + st]);
+          umma_commit(&b[L::H_SF + s_buf]);
+          if (ss.i == ss.last) umma_commit(&b[L::H_QE + q_buf]);
         }
-        ++i_s;
-        return true;
-      };
-      for (int k = 0; ok && k < NSB; ++k) ok = step_s();
-      int uv = 0, t = 0, n_o = 0;
-      uint32_t fixed = 0;  // parity of the next zeroing of each V slot
-      do {
-        bool first = true;
-        for (int i = pv.i0; ok && i < pv.i1; ++i, ++uv) {
-          const int st = uv % NSV;
-          const bool mine = pv.range.has(i);
-          const int r0 = pv.cur.s.L - pv.cur.it.tile(i) * BN;
-          const bool fix = r0 > 0 && r0 < BN && (r0 & (page_rows - 1)) != 0;
-          if (!mine) {
-            if (!(ok = wait_phase(&bars[L::B_VF + st], (uv / NSV) & 1, wd, 0x537))) break;
-            if (fix) fixed ^= 1u << st;
-            mbar_arrive(&bars[L::B_VE + st]);
-            ok = step_s();
-            continue;
-          }
-          if (!(ok = wait_phase(&b[L::H_PF + t % NSB], (t / NSB) & 1, wd, 0x538))) break;
-          if (first && !(ok = wait_phase(&b[L::H_OR + n_o % NOB], ((n_o / NOB) & 1) ^ 1, wd, 0x539))) break;
-          if (!(ok = wait_phase(&bars[L::B_VF + st], (uv / NSV) & 1, wd, 0x53a))) break;
-          if (fix) {
-            if (!(ok = wait_phase(&bars[L::B_VX + st], (fixed >> st) & 1, wd, 0x53b))) break;
-            fixed ^= 1u << st;
-          }
-          tc_fence_after();
-          const uint32_t tO = tS + L::TMEM_O + n_o % NOB * HD;
-          const uint32_t sv = sbase + L::OFF_V + st * L::KV_BYTES;
+        __syncwarp();
+        if (++s_buf == NSB) s_buf = 0;
+        if (ss.i == ss.last && ++q_buf == NQ) {
+          q_buf = 0;
+          q_ph ^= 1;
+        }
+      }
+      if (++k_st == NST) {
+        k_st = 0;
+        k_ph ^= 1;
+      }
+      ++ss.i;
+      return true;
+    };
+    bool ok = true;
+    for (int k = 0; ok && k < NSB; ++k) ok = step_s();
+    int v_st = 0, p_buf = 0, o_buf = 0;
+    uint32_t p_ph = 0, o_ph = 0, fixed = 0;  // fixed: parity of the next zeroing of each stage
+    bool more = ok;
+    while (more) {
+      Segment so = read(walks[1]);
+      bool first = true;
+      for (; so.i < so.i1; ++so.i) {
+        const bool on = so.has();
+        if (on) {
+          if (first) ok = warp_wait_phase(&b[L::H_OR + o_buf], o_ph ^ 1, wd, 0x539);
+          ok = ok && warp_wait_phase(&b[L::H_PF + p_buf], p_ph, wd, 0x538);
+        }
+        if (so.i == so.fix_at) {
+          ok = ok && warp_wait_phase(&bars[L::B_X + v_st], (fixed >> v_st) & 1, wd, 0x53b);
+          fixed ^= 1u << v_st;
+        }
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dv = dv0 + (v_st * L::KV_BYTES >> 4);
+        const uint32_t tO = tS + L::TMEM_O + o_buf * HD, tP = tS + p_buf * BN;
+        if (elect_one()) {
+          if (on) {
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            umma_f16_ts(tO, tS + t % NSB * BN + kk * 8, umma_sdesc_mn(sv + kk * 16 * L::ROW, L::KV_ATOM, kSbo, kSw),
-                        idesc_o, first && kk == 0 ? 0u : 1u);
-          first = false;
-          umma_commit(&bars[L::B_VE + st]);
-          umma_commit(&b[L::H_PE + t % NSB]);
-          if (i == pv.last) umma_commit(&b[L::H_OF + n_o++ % NOB]);
-          ++t;
-          ok = step_s();
+            for (int kk = 0; kk < BN / 16; ++kk)
+              umma_f16_ts(tO, tP + kk * 8, dv + (kk * 16 * L::ROW >> 4), idesc_o, kk == 0 && first ? 0u : 1u);
+            umma_commit(&bars[L::B_E + v_st]);
+            if (so.i == so.last) umma_commit(&b[L::H_OF + o_buf]);
+          } else {
+            mbar_arrive(&bars[L::B_E + v_st]);  // its stage was full before its scores were passed over
+          }
         }
-      } while (ok && pv.next(p, h, half_tokens, rpt));
-      // All MMAs this thread issued must finish before TMEM is released.
-      umma_commit(&b[L::H_DONE]);
-      wait_drain(&b[L::H_DONE], 0, kDrainLimitNs);
+        __syncwarp();
+        if (on) {
+          first = false;
+          if (++p_buf == NSB) {
+            p_buf = 0;
+            p_ph ^= 1;
+          }
+          if (so.i == so.last && ++o_buf == NOB) {
+            o_buf = 0;
+            o_ph ^= 1;
+          }
+        }
+        if (++v_st == NST) v_st = 0;
+        if (!(ok = step_s())) break;
+      }
+      more = ok && __shfl_sync(~0u, lane == 0 ? walks[1].next(p, rpt) : false, 0);
+      __syncwarp();
     }
+    // All MMAs the elected lane issued must finish before TMEM is released.
+    if (elect_one()) umma_commit(&b[L::H_DONE]);
+    __syncwarp();
+    if (lane == 0) wait_drain(&b[L::H_DONE], 0, kDrainLimitNs);
+    __syncwarp();
   } else if (warp >= 4 * NT) {
     if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_OTHER));
   } else {
@@ -461,21 +522,23 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     const float sl2 = p.scale_log2;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
     bool ok = true;
-    int t = 0, n_o = 0;
+    int s_buf = 0, o_buf = 0;
+    uint32_t s_ph = 0, o_ph = 0;
     // A finished segment's O is read after the next segment's first tile, by
     // when its last P.V has long completed.
     bool pend = false, pend_on = false;
     int pend_o = 0;
+    uint32_t pend_ph = 0;
     float pend_l = 0.f, pend_m = 0.f;
     T* pend_out = nullptr;      // whole item: the row of out
     float* pend_part = nullptr;  // cut item: its slot
     int pend_row = 0;
     auto finish = [&]() -> bool {
       pend = false;
-      if (!warp_wait_phase(&b[L::H_OF + pend_o % NOB], (pend_o / NOB) & 1, wd, 0x541)) return false;
+      if (!warp_wait_phase(&b[L::H_OF + pend_o], pend_ph, wd, 0x541)) return false;
       tc_fence_after();
-      const uint32_t tO = tS + L::TMEM_O + pend_o % NOB * HD;
-      const float inv = pend_l > 0.f ? 1.f / pend_l : 0.f;
+      const uint32_t tO = tS + L::TMEM_O + pend_o * HD;
+      const float inv = pend_l > 1e-30f ? 1.f / pend_l : 0.f;  // (a row that sees a key has l >= 1)
       if (pend_on && pend_part) {
         pend_part[L::ROWS * HD + pend_row] = pend_m;
         pend_part[L::ROWS * HD + L::ROWS + pend_row] = pend_l;
@@ -510,28 +573,46 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&b[L::H_OR + pend_o % NOB]);
+      if (lane == 0) mbar_arrive(&b[L::H_OR + pend_o]);
       return true;
     };
 
-    walk.cur.seek(p, start.b, start.off, rpt);
-    walk.left = n_units;
-    walk.load(p, h, half_tokens);
-    do {
-      const bool on = row < walk.rows;
+    // The walk rests in shared memory while a segment is worked on: its
+    // registers would push the scores out.
+    if (lane == 0) saved[warp].begin(p, start, n_units, rpt);
+    bool more = true;
+    int units = 0;  // of the segments so far
+    for (; ok && more; more = __shfl_sync(~0u, lane == 0 ? saved[warp].next(p, rpt) : false, 0)) {
+      ChunkRange range;
+      int i, last, p0, p1, pos, n_sink, w_shift, unit;  // unit: ring position of tile i
+      bool on;
       const int item_row = h * half_rows + row;
-      const int pos = walk.p0 + row / p.group;
-      const bool cut = walk.i0 > 0 || walk.i1 < walk.cur.it.n;
       T* out = nullptr;
-      float* part = nullptr;
-      if (on) {
-        const int r = walk.cur.it.r0 + item_row;
-        const long long tok = walk.cur.s.q0 + r / p.group;
-        out = static_cast<T*>(p.out) + (tok * p.heads + walk.cur.kvh * p.group + r % p.group) * p.out_hd;
+      float* part = nullptr;  // set when the item is cut
+      __syncwarp();           // lane 0's walk is visible
+      {
+        const ChunkWalk<HD>& w = saved[warp];
+        const ChunkHalf x = w.half(p, h, half_tokens);
+        range = x.range;
+        i = w.i0 < range.a ? w.i0 : max(range.c, w.i0);
+        last = x.last;
+        unit = units + i - w.i0;
+        units += w.i1 - w.i0;
+        p0 = x.p0;
+        p1 = x.p1;
+        pos = x.p0 + row / p.group;
+        on = row < x.rows;
+        n_sink = w.cur.it.n_sink;
+        w_shift = w.cur.it.w_tile - n_sink;
+        const int r = w.cur.it.r0 + item_row;
+        const long long tok = w.cur.s.q0 + r / p.group;
+        if (on) out = static_cast<T*>(p.out) + (tok * p.heads + w.cur.kvh * p.group + r % p.group) * p.out_hd;
+        if (w.i0 > 0 || w.i1 < w.cur.it.n)
+          part = p.part + (2ll * blockIdx.x + (w.i0 > 0 ? 0 : 1)) * paged_slot_floats<L::ROWS, HD>();
       }
-      if (cut) part = p.part + (2ll * blockIdx.x + (walk.i0 > 0 ? 0 : 1)) * paged_slot_floats<L::ROWS, HD>();
-      if (walk.last < 0) {  // nothing here for this half
-        if (on && cut) {
+      __syncwarp();  // read before lane 0 moves it on
+      if (last < 0) {  // nothing here for this half
+        if (on && part) {
           part[L::ROWS * HD + item_row] = -INFINITY;
           part[L::ROWS * HD + L::ROWS + item_row] = 0.f;
           for (int d = 0; d < HD; d += 4) *reinterpret_cast<float4*>(part + item_row * HD + d) = make_float4(0, 0, 0, 0);
@@ -540,31 +621,31 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         }
         continue;
       }
-      const uint32_t tO = tS + L::TMEM_O + n_o % NOB * HD;
+      // Every row of the half sees all of a tile that starts at k0 <= k_hi
+      // and, under a window, past k_lo or within the first tokens.
+      const int k_hi = p0 - BN + 1, k_lo = p.window > 0 ? p1 - p.window : -1, k_sk = p.sinks - BN;
+      const int lo_pos = p.window > 0 ? pos - p.window + 1 : 0;
+      const uint32_t tO = tS + L::TMEM_O + o_buf * HD;
       float m_run = -INFINITY, l_run = 0.f;
+      int prev = 0;  // ring position of the tile before
       bool first = true;
-      for (int i = walk.i0; ok && i <= walk.last; ++i) {
-        if (!walk.range.has(i)) {
-          if (i >= walk.range.a && i < walk.range.c) i = max(walk.range.c, walk.i0) - 1;  // over the gap
-          continue;
-        }
-        const int bb = t % NSB, k0 = walk.cur.it.tile(i) * BN;
-        // Warp-uniform: some row of the half does not see the whole tile.
-        const bool masked = !(k0 + BN - 1 <= walk.p0 &&
-                              (p.window == 0 || k0 > walk.p1 - p.window || k0 + BN <= p.sinks));
-        if (!(ok = warp_wait_phase(&b[L::H_SF + bb], (t / NSB) & 1, wd, 0x542))) break;
+      for (;;) {
+        const int k0 = (i < n_sink ? i : i + w_shift) * BN;
+        const bool masked = k0 > k_hi || (k0 <= k_lo && k0 > k_sk);  // warp-uniform
+        if (!(ok = warp_wait_phase(&b[L::H_SF + s_buf], s_ph, wd, 0x542))) break;
         tc_fence_after();
+        const uint32_t tSb = tS + s_buf * BN;
         uint32_t sc[BN / 32][32];
 #pragma unroll
-        for (int g = 0; g < BN / 32; ++g) tmem_ld_x32(tS + bb * BN + 32 * g, sc[g]);
+        for (int g = 0; g < BN / 32; ++g) tmem_ld_x32(tSb + 32 * g, sc[g]);
 #pragma unroll
         for (int g = 0; g < BN / 32; ++g) tmem_ld_wait_tied(sc[g]);
         if (masked) {
-          const int hi = pos - k0 + 1, lo = p.window > 0 ? pos - p.window + 1 - k0 : 0, sk = p.sinks - k0;
+          const int hi = pos - k0 + 1, lo = lo_pos - k0, sk = p.sinks - k0;
 #pragma unroll
           for (int g = 0; g < BN / 32; ++g) {
-            const uint32_t see = bits_below(hi - 32 * g) &
-                                 (p.window > 0 ? ~bits_below(lo - 32 * g) | bits_below(sk - 32 * g) : ~0u);
+            const uint32_t see =
+                bits_below(hi - 32 * g) & (~bits_below(lo - 32 * g) | bits_below(sk - 32 * g));
             if (see != ~0u) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
@@ -594,9 +675,8 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         }
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
         if (__any_sync(~0u, resc)) {
-          // O must hold every earlier tile (with one S buffer it does: S of this tile was issued after P.V of the last).
-          if constexpr (NSB > 1)
-            if (!(ok = warp_wait_phase(&b[L::H_PE + (t - 1) % NSB], ((t - 1) / NSB) & 1, wd, 0x543))) break;
+          // O must hold every earlier tile: P.V of the last one hands its stage back.
+          if (!(ok = warp_wait_phase(&bars[L::B_E + prev % NST], (prev / NST) & 1, wd, 0x543))) break;
           tc_fence_after();
           const float corr = resc ? ex2_approx(m_run - m_new) : 1.f;
           l_run *= corr;
@@ -614,53 +694,60 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         const uint64_t negm = f2_pack(-m_use, -m_use);
         const float y_scale = sl2 * kExpYScale, y_bias = fmaf(-m_use, kExpYScale, kExpYBias);
         uint64_t sum[2] = {f2_pack(l_run, 0.f), 0ull};
-        // POLY of every 8 pairs take the polynomial; none in a masked tile,
-        // where a hidden score must give exactly 0 and the clamp would not.
-        auto probabilities = [&](auto poly) {
-          constexpr int POLY = decltype(poly)::value;
+        // A hidden score gives 0 on MUFU and 2^-126 where the polynomial's
+        // clamp ends: nothing beside the row's largest term, which is at least
+        // 1, and a row that saw no key is known by its tiny sum.
 #pragma unroll
-          for (int g = 0; g < BN / 32; ++g) {
-            uint32_t pk[16];
+        for (int g = 0; g < BN / 32; ++g) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              uint64_t pp;
-              const float s0 = __uint_as_float(sc[g][2 * e]), s1 = __uint_as_float(sc[g][2 * e + 1]);
-              if ((e & 7) < POLY) {
-                pp = exp2_pair_wide(f2_pack(fma_sat(s0, y_scale, y_bias), fma_sat(s1, y_scale, y_bias)));
-              } else {
-                const uint64_t xx = ffma2(f2_pack(s0, s1), sl2x2, negm);
-                pp = f2_pack(ex2_approx(f2_lo(xx)), ex2_approx(f2_hi(xx)));
-              }
-              sum[e & 1] = fadd2(sum[e & 1], pp);
-              pk[e] = PT::pack(f2_lo(pp), f2_hi(pp));
+          for (int e = 0; e < 16; ++e) {
+            uint64_t pp;
+            const float s0 = __uint_as_float(sc[g][2 * e]), s1 = __uint_as_float(sc[g][2 * e + 1]);
+            if ((e & 7) < kChunkExpFma<HD>) {
+              pp = exp2_pair_wide(f2_pack(fma_sat(s0, y_scale, y_bias), fma_sat(s1, y_scale, y_bias)));
+            } else {
+              const uint64_t xx = ffma2(f2_pack(s0, s1), sl2x2, negm);
+              pp = f2_pack(ex2_approx(f2_lo(xx)), ex2_approx(f2_hi(xx)));
             }
-            tmem_st_x16(tS + bb * BN + 16 * g, pk);
+            sum[e & 1] = fadd2(sum[e & 1], pp);
+            pk[e] = PT::pack(f2_lo(pp), f2_hi(pp));
           }
-        };
-        if (masked)
-          probabilities(std::integral_constant<int, 0>());
-        else
-          probabilities(std::integral_constant<int, kChunkExpFma<HD>>());
+          tmem_st_x16(tSb + 16 * g, pk);
+        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&b[L::H_PF + bb]);
+        if (lane == 0) mbar_arrive(&b[L::H_PF + s_buf]);
         const uint64_t both = fadd2(sum[0], sum[1]);
         l_run = f2_lo(both) + f2_hi(both);
-        ++t;
+        if (++s_buf == NSB) {
+          s_buf = 0;
+          s_ph ^= 1;
+        }
         if (first && pend && !(ok = finish())) break;
         first = false;
+        prev = unit;
+        const int next = i + 1 >= range.a && i + 1 < range.c ? range.c : i + 1;
+        unit += next - i;
+        i = next;
+        if (i > last) break;
       }
       if (!ok) break;
       pend = true;
       pend_on = on;
-      pend_o = n_o++;
+      pend_o = o_buf;
+      pend_ph = o_ph;
       pend_l = l_run;
       pend_m = m_run;
       pend_out = out;
-      pend_part = cut ? part : nullptr;
+      pend_part = part;
       pend_row = item_row;
-    } while (walk.next(p, h, half_tokens, rpt));
+      if (++o_buf == NOB) {
+        o_buf = 0;
+        o_ph ^= 1;
+      }
+    }
     if (ok && pend) ok = finish();
   }
 
