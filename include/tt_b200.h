@@ -206,7 +206,7 @@ typedef struct tt_kv_cache {
   int page;                /* tokens per page: 16, 32, 64, 128 or 256 */
   int head_dim;            /* as stored: 16, 32, 64, 128 or 256 */
   int n_slots;
-  int table_width;
+  int table_width;         /* table_width * page < 2^30 */
 } tt_kv_cache;
 
 /* Makes room for the new tokens of a batch of distinct slots: allocates the
@@ -258,7 +258,8 @@ int tt_cache_copy_pages(const tt_kv_cache* cache, const int* src, const int* dst
  * for a row that sees none and for a row of no sequence; FP32 statistics and
  * accumulation, out in the cache's type.  q: [n_tokens, heads, stored
  * head_dim], element strides token and head, multiples of 8; query head h
- * reads KV head h / (heads / kv_heads), heads / kv_heads <= 128.  head_dim: 8
+ * reads KV head h / (heads / kv_heads), heads / kv_heads <= 128; fewer than
+ * 2^30 query rows (tokens times heads / kv_heads).  head_dim: 8
  * (stored 16 wide), 16, 32, 64, 128 or 256.  max_q_len: an upper bound of T
  * (<= 0: n_tokens).  is_bf16: type of q, the pages and out (0: FP16).
  * workspace: tt_paged_attention_workspace_bytes. */

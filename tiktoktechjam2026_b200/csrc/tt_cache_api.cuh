@@ -34,8 +34,8 @@ int cache_params(const tt_kv_cache* c, bool values, bool counts, CacheParams* ou
   if (c->n_slots <= 0 || c->table_width <= 0 || c->n_pages <= 0 || c->table_stride < c->table_width)
     return fail(TT_ERR_SHAPE, "invalid slots, table width, table stride or pages (%d, %d, %lld, %d)", c->n_slots,
                 c->table_width, static_cast<long long>(c->table_stride), c->n_pages);
-  if (static_cast<long long>(c->table_width) * c->page > 0x7fffffffLL)
-    return fail(TT_ERR_SHAPE, "table rows of %d pages of %d tokens pass 2^31 tokens", c->table_width, c->page);
+  if (static_cast<long long>(c->table_width) * c->page >= 1LL << 30)
+    return fail(TT_ERR_SHAPE, "table rows of %d pages of %d tokens reach 2^30 tokens", c->table_width, c->page);
   memset(out, 0, sizeof(*out));
   out->tables = c->tables;
   out->table_stride = c->table_stride;
@@ -73,9 +73,9 @@ int cache_params(const tt_kv_cache* c, bool values, bool counts, CacheParams* ou
 // Sequences of at most this many query rows (tokens * group) take the kernel
 // for short chunks, whose items hold that many rows.
 constexpr int kRowsMax = 16;
-// Units that a worker takes at least: fewer would cost more in joining than
-// the shorter pieces save.
-constexpr long long kRowsMinUnits = 2, kChunkMinUnits = 4;
+// Key tiles that a worker takes at least: shorter pieces would cost more in
+// joining than they save.
+constexpr int kRowsMinTiles = 2, kChunkMinTiles = 4;
 
 template <int HD>
 size_t paged_part_bytes(int sm_count) {
@@ -96,6 +96,15 @@ int paged_workspace(int hd, int sm_count, size_t* bytes) {
   }
 }
 
+template <typename T, int HD, int TK, int ROWS, int RB>
+int launch_paged_join(const PagedParams& p, int tpi, int min_tiles, cudaStream_t stream) {
+  if (p.n_workers > kPagedMaxWorkers) return fail(TT_ERR_UNSUPPORTED, "%d workers", p.n_workers);
+  PdlScope programmatic;
+  launch_kernel(paged_join_kernel<T, HD, TK, ROWS, RB>, dim3(p.n_workers - 1, ROWS / RB), kJoinThreads, 0, stream, p,
+                tpi, min_tiles);
+  return after_launch("paged attention join");
+}
+
 // Sequences of row_lo .. row_hi query rows.
 template <typename T, int HD>
 int launch_paged_rows(PagedParams p, int row_lo, int row_hi, int sm_count, cudaStream_t stream) {
@@ -105,11 +114,9 @@ int launch_paged_rows(PagedParams p, int row_lo, int row_hi, int sm_count, cudaS
   p.row_lo = row_lo;
   p.row_hi = row_hi;
   p.n_workers = sm_count * L::WARPS;
-  launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, p, kRowsMinUnits);
+  launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, p, kRowsMax / p.group, kRowsMinTiles);
   if (int rc = after_launch("paged attention (rows)")) return rc;
-  launch_kernel(paged_join_kernel<T, HD, L::TK, kRowsMax, kRowsMax, 256>, p.n_workers - 1, 256, 0, stream, p, kRowsMax,
-                kRowsMinUnits);
-  return after_launch("paged attention join");
+  return launch_paged_join<T, HD, L::TK, kRowsMax, kRowsMax>(p, kRowsMax / p.group, kRowsMinTiles, stream);
 }
 
 template <typename T, int HD>
@@ -138,12 +145,9 @@ int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t str
     const uint32_t box[3] = {L::ATOM, static_cast<uint32_t>(page < L::BN ? page : L::BN), 1};
     if (int rc = encode_f16(kv ? &tv : &tk, kv ? p.v_pages : p.k_pages, 3, dims, strides, box)) return rc;
   }
-  launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, tq, tk, tv, p, half_tokens, kChunkMinUnits);
+  launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, tq, tk, tv, p, half_tokens, kChunkMinTiles);
   if (int rc = after_launch("paged attention (chunk)")) return rc;
-  constexpr int RB = 32;
-  launch_kernel(paged_join_kernel<T, HD, L::BN, L::ROWS, RB, 256>, dim3(sm_count - 1, L::ROWS / RB), 256, 0, stream, p,
-                L::NT * half_tokens * p.group, kChunkMinUnits);
-  return after_launch("paged attention join");
+  return launch_paged_join<T, HD, L::BN, L::ROWS, 32>(p, L::NT * half_tokens, kChunkMinTiles, stream);
 }
 
 // Each sequence goes by its own number of query rows; max_rows only saves
@@ -151,6 +155,11 @@ int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t str
 template <typename T, int HD>
 int launch_paged(const PagedParams& p, int max_rows, int sm_count, cudaStream_t stream) {
   if (max_rows <= kRowsMax) return launch_paged_rows<T, HD>(p, 0, 0x7fffffff, sm_count, stream);
+  // With few (sequence, KV head) pairs the chunk kernel takes short sequences
+  // along, at most two per SM: that costs less than a second pair of launches
+  // (SEE_LOG).
+  if (p.group > kRowsMax || static_cast<long long>(p.batch) * p.kv_heads <= 2ll * sm_count)
+    return launch_paged_chunk<T, HD>(p, 0, sm_count, stream);
   if (int rc = launch_paged_chunk<T, HD>(p, kRowsMax + 1, sm_count, stream)) return rc;
   return launch_paged_rows<T, HD>(p, 0, kRowsMax, sm_count, stream);
 }
@@ -323,7 +332,7 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
     if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || q_token_stride % 8 != 0 || q_head_stride % 8 != 0)
       return fail(TT_ERR_ALIGN, "q, out and workspace must be 16-byte aligned, q's strides multiples of 8");
     const int group = heads / c.kv_heads;
-    if (static_cast<long long>(n_tokens) * group > 0x7fffffffLL) return fail(TT_ERR_SHAPE, "too many query rows");
+    if (static_cast<long long>(n_tokens) * group >= 1LL << 30) return fail(TT_ERR_SHAPE, "too many query rows");
     if (n_tokens == 0) return TT_OK;
     PagedParams p;
     memset(&p, 0, sizeof(p));
@@ -350,8 +359,9 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
     p.n_pages = c.n_pages;
     p.page_shift = c.page_shift;
     p.table_width = c.table_width;
-    p.window = window;
-    p.sinks = sinks;
+    const int room = c.table_width << c.page_shift;  // no position reaches it
+    p.window = window < room ? window : 0;
+    p.sinks = sinks < room ? sinks : room;
     p.out_hd = head_dim;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.err = ds->err;

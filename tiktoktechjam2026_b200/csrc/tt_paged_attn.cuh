@@ -9,14 +9,15 @@
 //   o = sum_u 2^(s_u - m) v_u / sum_u 2^(s_u - m),  s_u = (q . k_u) scale log2 e.
 // A row that sees no key (t < 0) is zero, and so is a row of no sequence.
 //
-// Work is measured in units of one key tile of one item (a tile of query rows
-// of one sequence and KV head).  All units of the call form one line, cut into
-// equal pieces, one per worker: a worker's piece may begin and end inside an
-// item, so a single long sequence and a ragged batch both fill the GPU.  An
-// item that lies in one piece is finished by its worker; the parts of an item
-// that was cut (O unnormalised, m, l, in FP32) go to the workspace and are
-// joined by paged_join_kernel, always in worker order, so results do not
-// depend on timing.
+// Work is laid out on one line: an item (some tokens of one sequence for one KV
+// head) takes as much of it as its queries span keys, plus a constant.  The
+// line is cut into equal pieces, one per worker, and a cut inside an item falls
+// on a key tile, so a single long sequence and a ragged batch both fill the
+// GPU.  Sums over the items of a sequence are closed forms: no kernel walks
+// items to find its piece.  An item that lies in one piece is finished by its
+// worker; the parts of an item that was cut (O unnormalised, m, l, in FP32) go
+// to the workspace and are joined by paged_join_kernel, always in worker order,
+// so results do not depend on timing.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -68,18 +69,24 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
   return s;
 }
 
-// One item: RPT query rows (row = token * group + head of the group) of one
-// sequence, and the key tiles that some row of it can see.  With a window the
+constexpr int kPagedMaxWorkers = 2048;
+
+// Extra length of an item on the line, in key tiles: its queries' loads and its output.
+constexpr int kPagedItemTiles = 2;
+
+// One item: the tokens qt * tpi .. of a sequence (rows: token * group + head of
+// the group) and the key tiles that some row of it can see.  With a window the
 // tiles are [0, n_sink) and [w_tile, ...); tile(i) maps the i-th of n.
 template <int TK>
 struct PagedItem {
-  int r0, rows, p0, p1;  // first row, rows, positions of the first and last row's token
+  int r0, rows, p0, p1;  // first row, rows, positions of the first and last token
   int n, n_sink, w_tile;
-  __device__ __forceinline__ void set(const PagedParams& p, const PagedSeq& s, int qt, int rpt) {
-    r0 = qt * rpt;
-    rows = min(rpt, s.T * p.group - r0);
-    p0 = s.L - s.T + r0 / p.group;
-    p1 = s.L - s.T + (r0 + rows - 1) / p.group;
+  __device__ __forceinline__ void set(const PagedParams& p, const PagedSeq& s, int qt, int tpi) {
+    const int t0 = qt * tpi, t1 = min(t0 + tpi, s.T);
+    r0 = t0 * p.group;
+    rows = (t1 - t0) * p.group;
+    p0 = s.L - s.T + t0;
+    p1 = s.L - s.T + t1 - 1;
     const int total = p1 < 0 ? 1 : p1 / TK + 1;  // an item of rows that see nothing keeps one tile, wholly masked
     n_sink = total;
     w_tile = total;
@@ -91,8 +98,7 @@ struct PagedItem {
       if (ns < wt) {
         n_sink = ns;
         w_tile = wt;
-        n = ns + max(total - wt, 0);
-        if (n == 0) n = 1;
+        n = ns + total - wt;
       }
     }
   }
@@ -103,104 +109,143 @@ struct PagedItem {
   }
 };
 
-__device__ __forceinline__ int paged_q_tiles(const PagedParams& p, const PagedSeq& s, int rpt) {
+__device__ __forceinline__ int paged_q_tiles(const PagedParams& p, const PagedSeq& s, int tpi) {
   const int rows = s.T * p.group;
-  return rows >= p.row_lo && rows <= p.row_hi ? (rows + rpt - 1) / rpt : 0;
+  return rows >= p.row_lo && rows <= p.row_hi ? (s.T + tpi - 1) / tpi : 0;
 }
 
-// Units of sequence b for one KV head.
-template <int TK>
-__device__ __forceinline__ long long paged_head_units(const PagedParams& p, const PagedSeq& s, int rpt) {
-  const int nq = paged_q_tiles(p, s, rpt);
-  long long u = 0;
-  PagedItem<TK> it;
-  for (int qt = 0; qt < nq; ++qt) {
-    it.set(p, s, qt, rpt);
-    u += it.n;
-  }
-  return u;
+// sum over j < n of max(a + j d, 0), d > 0.
+__device__ __forceinline__ long long ramp_sum(long long a, int d, int n) {
+  const int j0 = a >= 0 ? 0 : static_cast<int>(min((-a + d - 1) / d, static_cast<long long>(n)));
+  const long long m = n - j0;
+  return m * (a + static_cast<long long>(j0) * d) + d * (m * (m - 1) / 2);
 }
 
-// Walks the units of one worker's piece: sequence, KV head, query tile, tile.
+// Length on the line of the first q of sequence s's nq items for one KV head:
+// item j spans the keys up to position p1(j), less, under a window, those
+// between the first tokens and the window of p0(j).
 template <int TK>
-struct PagedCursor {
-  int b, kvh, qt, nq, i;
-  PagedSeq s;
-  PagedItem<TK> it;
-  __device__ __forceinline__ void open(const PagedParams& p, int rpt) {  // enters sequence b, or the next with work
-    while (b < p.batch) {
-      s = paged_seq(p, b);
-      nq = paged_q_tiles(p, s, rpt);
-      if (nq > 0) {
-        it.set(p, s, 0, rpt);
-        return;
-      }
-      ++b;
-    }
-  }
-  // Places the cursor `off` units into sequence b.
-  __device__ __forceinline__ void seek(const PagedParams& p, int b_, long long off, int rpt) {
-    b = b_;
-    s = paged_seq(p, b);
-    nq = paged_q_tiles(p, s, rpt);
-    const long long per_head = paged_head_units<TK>(p, s, rpt);
-    kvh = static_cast<int>(off / per_head);
-    off -= kvh * per_head;
-    qt = 0;
-    it.set(p, s, 0, rpt);
-    while (off >= it.n) {
-      off -= it.n;
-      it.set(p, s, ++qt, rpt);
-    }
-    i = static_cast<int>(off);
-  }
-  __device__ __forceinline__ void next_item(const PagedParams& p, int rpt) {
-    i = 0;
-    if (++qt < nq) {
-      it.set(p, s, qt, rpt);
-      return;
-    }
-    qt = 0;
-    if (++kvh < p.kv_heads) {
-      it.set(p, s, 0, rpt);
-      return;
-    }
-    kvh = 0;
-    ++b;
-    open(p, rpt);
-  }
-};
+__device__ __forceinline__ long long paged_line(const PagedParams& p, const PagedSeq& s, int q, int nq, int tpi) {
+  if (q == 0) return 0;
+  const long long base = s.L - s.T;
+  const int whole = q == nq ? q - 1 : q;  // the last item may hold fewer tokens
+  long long len = static_cast<long long>(q) * (kPagedItemTiles * TK) + ramp_sum(base + tpi, tpi, whole);
+  if (q == nq) len += s.L;
+  if (p.window > 0) len -= ramp_sum(base - p.window + 1 - p.sinks, tpi, q);
+  return len;
+}
 
-// Where a worker's piece begins: sequence and units into it (b < 0: no work).
-struct PagedStart {
+// A cut of the line: sequence and length into it (b < 0: the end of the line).
+struct PagedCut {
   int b;
   long long off;
 };
 
-// Block-wide: total units, units per worker, and the start of the workers
-// first_worker .. first_worker + NW - 1 (fewer than 32).  Every thread takes part.
-template <int TK, int NW, int THREADS>
-__device__ __forceinline__ void paged_schedule(const PagedParams& p, int rpt, long long min_units, int first_worker,
-                                               PagedStart* starts, long long* total, long long* per) {
+// Walks one worker's piece item by item: sequence, KV head, item, tiles i .. i1.
+template <int TK>
+struct PagedWalk {
+  int b, kvh, qt, nq, i, i1;
+  PagedSeq s;
+  PagedItem<TK> it;
+  int end_b, end_kvh, end_qt, end_i;
+  long long start, len;  // seek: the line before the item within (sequence, KV head), and the item's length
+
+  __device__ __forceinline__ void seek(const PagedParams& p, const PagedCut& c, int tpi) {
+    b = c.b;
+    s = paged_seq(p, b);
+    nq = paged_q_tiles(p, s, tpi);
+    const long long head = paged_line<TK>(p, s, nq, nq, tpi);
+    kvh = static_cast<int>(c.off / head);
+    const long long off = c.off - kvh * head;
+    int lo = 0, hi = nq;  // the last item that begins at or before off
+    start = 0;
+    long long next = head;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      const long long x = paged_line<TK>(p, s, mid, nq, tpi);
+      if (x <= off) {
+        lo = mid;
+        start = x;
+      } else {
+        hi = mid;
+        next = x;
+      }
+    }
+    qt = lo;
+    len = next - start;
+    it.set(p, s, qt, tpi);
+    i = tile_at(off - start);
+  }
+  // The tile on which a cut at length x of the item falls.
+  __device__ __forceinline__ int tile_at(long long x) const { return static_cast<int>(x * it.n / len); }
+
+  __device__ __forceinline__ bool at_end() const { return b == end_b && kvh == end_kvh && qt == end_qt; }
+  // Whether the piece from cut c to cut e holds any tile; places the walk on its first.
+  __device__ __forceinline__ bool begin(const PagedParams& p, const PagedCut& c, const PagedCut& e, int tpi) {
+    end_b = p.batch;
+    if (c.b < 0) return false;
+    if (e.b >= 0) {
+      seek(p, e, tpi);
+      end_b = b;
+      end_kvh = kvh;
+      end_qt = qt;
+      end_i = i;
+    }
+    seek(p, c, tpi);
+    i1 = at_end() ? end_i : it.n;
+    return i < i1;
+  }
+  // On to the next item; false at the end of the piece.
+  __device__ __forceinline__ bool next(const PagedParams& p, int tpi) {
+    if (at_end()) return false;
+    i = 0;
+    if (++qt == nq) {
+      qt = 0;
+      if (++kvh == p.kv_heads) {
+        kvh = 0;
+        do {
+          if (++b >= p.batch) return false;
+          s = paged_seq(p, b);
+          nq = paged_q_tiles(p, s, tpi);
+        } while (nq == 0);
+      }
+    }
+    it.set(p, s, qt, tpi);
+    i1 = at_end() ? end_i : it.n;
+    return i1 > 0;
+  }
+};
+
+// Block-wide: the piece length `per` and the cuts where the workers
+// first_worker .. first_worker + NC - 1 begin (NC < 32).  Every thread takes part.
+template <int TK, int NC, int THREADS>
+__device__ __forceinline__ void paged_schedule(const PagedParams& p, int tpi, int min_tiles, int first_worker,
+                                               PagedCut* cuts, long long* per) {
   constexpr int NWARPS = THREADS / 32;
   __shared__ long long warp_sum[NWARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  long long sum = 0;
-  for (int b = tid; b < p.batch; b += THREADS) sum += paged_head_units<TK>(p, paged_seq(p, b), rpt) * p.kv_heads;
+  auto length = [&](int b) -> long long {
+    if (b >= p.batch) return 0;
+    const PagedSeq s = paged_seq(p, b);
+    const int nq = paged_q_tiles(p, s, tpi);
+    return paged_line<TK>(p, s, nq, nq, tpi) * p.kv_heads;
+  };
+  const long long mine = length(tid);  // kept for the scan below: most batches are one round
+  long long sum = mine;
+  for (int b = tid + THREADS; b < p.batch; b += THREADS) sum += length(b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
   if (lane == 0) warp_sum[warp] = sum;
-  if (tid < NW) starts[tid].b = -1;
+  if (tid < NC) cuts[tid].b = -1;
   __syncthreads();
   long long all = 0;
   for (int w = 0; w < NWARPS; ++w) all += warp_sum[w];
-  const long long each = max((all + p.n_workers - 1) / p.n_workers, min_units);
-  *total = all;
+  const long long each = max((all + p.n_workers - 1) / p.n_workers, static_cast<long long>(min_tiles) * TK);
   *per = each;
   long long carry = 0;
   for (int b0 = 0; b0 < p.batch && all > 0; b0 += THREADS) {
     const int b = b0 + tid;
-    const long long u = b < p.batch ? paged_head_units<TK>(p, paged_seq(p, b), rpt) * p.kv_heads : 0;
+    const long long u = b0 == 0 ? mine : length(b);
     long long inc = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -214,9 +259,9 @@ __device__ __forceinline__ void paged_schedule(const PagedParams& p, int rpt, lo
     for (int w = 0; w < warp; ++w) before += warp_sum[w];
     for (int w = 0; w < NWARPS; ++w) carry += warp_sum[w];
     const long long lo = before + inc - u, hi = before + inc;
-    for (int w = 0; w < NW; ++w) {
-      const long long start = (first_worker + w) * each;
-      if (start >= lo && start < hi) starts[w] = {b, start - lo};
+    for (int w = 0; w < NC; ++w) {
+      const long long cut = (first_worker + w) * each;
+      if (cut >= lo && cut < hi) cuts[w] = {b, cut - lo};
     }
   }
   __syncthreads();
@@ -292,49 +337,95 @@ __host__ __device__ constexpr long long paged_slot_floats() {
 // Joins the parts of the item that the start of worker c cuts, if c is the
 // first worker to start inside it: with M = max_i m_i,
 //   O = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
-// One block per (worker, RB rows of the item); a thread per two features.
-template <typename T, int HD, int TK, int ROWS, int RB, int THREADS>
-__global__ void __launch_bounds__(THREADS) paged_join_kernel(const PagedParams p, int rpt, long long min_units) {
-  __shared__ PagedStart start;
-  long long total, per;
+// One block per (worker, RB rows of the item).  A thread has four features of a
+// row; where rows are few, the parts are dealt over several threads and their
+// sums joined in a fixed order.  All blocks are resident at once, and most only
+// find that they have nothing to join: the schedule runs before the kernel
+// whose parts it reads has ended (programmatic launch).
+constexpr int kJoinThreads = 256;
+
+struct JoinSum {
+  float m, l;
+  float4 o;
+  __device__ __forceinline__ void add(float mk, float lk, const float4& ok) {
+    const float top = fmaxf(m, mk), base = top == -INFINITY ? 0.f : top;
+    const float a = ex2_approx(m - base), b = ex2_approx(mk - base);
+    m = top;
+    l = l * a + lk * b;
+    o.x = o.x * a + ok.x * b;
+    o.y = o.y * a + ok.y * b;
+    o.z = o.z * a + ok.z * b;
+    o.w = o.w * a + ok.w * b;
+  }
+};
+
+template <typename T, int HD, int TK, int ROWS, int RB>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedParams p, int tpi, int min_tiles) {
+  __shared__ PagedCut cuts[2];
+  __shared__ uint8_t holds[kPagedMaxWorkers];  // whether the k-th worker from c on has a part
+  __shared__ JoinSum sums[kJoinThreads];
+  long long per;
   const int c = blockIdx.x + 1;  // worker 0 starts at an item's beginning
+  paged_schedule<TK, 2, kJoinThreads>(p, tpi, min_tiles, c - 1, cuts, &per);
+  if (cuts[1].b < 0) return;
+  PagedWalk<TK> cur;
+  cur.seek(p, cuts[1], tpi);
+  const int row0 = blockIdx.y * RB, rows = min(cur.it.rows - row0, RB);
+  if (cur.i == 0 || rows <= 0) return;
+  // Length into the item at which worker c starts; the others lie `per` apart.
+  const long long at = cuts[1].off - cur.kvh * paged_line<TK>(p, cur.s, cur.nq, cur.nq, tpi) - cur.start;
+  if (at > per && cur.tile_at(at - per) > 0) return;  // worker c - 1 starts inside too
+  const int n_after = static_cast<int>((cur.len - at + per - 1) / per);  // workers c .. that start inside
+  for (int k = threadIdx.x; k < n_after; k += kJoinThreads)
+    holds[k] = cur.tile_at(at + k * per) < (k + 1 < n_after ? cur.tile_at(at + (k + 1) * per) : cur.it.n);
+  __syncthreads();
   pdl_wait();
-  pdl_trigger();
-  paged_schedule<TK, 1, THREADS>(p, rpt, min_units, c, &start, &total, &per);
-  if (start.b < 0) return;
-  PagedCursor<TK> cur;
-  cur.seek(p, start.b, start.off, rpt);
-  if (cur.i == 0 || cur.i > per) return;  // starts with the item, or an earlier worker starts inside it
-  const long long end = static_cast<long long>(c) * per - cur.i + cur.it.n;  // one past the item's last unit
-  const int n_after = static_cast<int>((end - 1) / per) - c + 1;             // workers c .. that hold a part
   constexpr long long SLOT = paged_slot_floats<ROWS, HD>();
   const float* first = p.part + (2ll * (c - 1) + 1) * SLOT;
   const float* rest = p.part + 2ll * c * SLOT;  // then every 2 SLOT
-  constexpr int TPR = HD / 2;                   // threads of one row
-  for (int x = threadIdx.x; x < RB * TPR; x += THREADS) {
-    const int row = blockIdx.y * RB + x / TPR, d = x % TPR * 2;
-    if (row >= cur.it.rows || d >= p.out_hd) continue;
-    const int o_at = row * HD + d, m_at = ROWS * HD + row, l_at = m_at + ROWS;
-    float m = first[m_at];
-    for (int k = 0; k < n_after; ++k) m = fmaxf(m, rest[2 * SLOT * k + m_at]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float w = ex2_approx(first[m_at] - base);
-    float l = first[l_at] * w;
-    const float2 o0 = *reinterpret_cast<const float2*>(first + o_at);
-    float a0 = o0.x * w, a1 = o0.y * w;
-    for (int k = 0; k < n_after; ++k) {
-      const float* s = rest + 2 * SLOT * k;
-      w = ex2_approx(s[m_at] - base);
-      l = fmaf(s[l_at], w, l);
-      const float2 o = *reinterpret_cast<const float2*>(s + o_at);
-      a0 = fmaf(o.x, w, a0);
-      a1 = fmaf(o.y, w, a1);
+  constexpr int TPR = HD / 4, GROUPS = kJoinThreads / TPR;
+  const int g = threadIdx.x / TPR, d = threadIdx.x % TPR * 4;
+  const int deal = rows < GROUPS ? GROUPS / rows : 1;  // threads over which a row's parts are dealt
+  for (int r0 = 0; r0 < rows; r0 += GROUPS) {
+    const int row = row0 + r0 + g % min(rows, GROUPS), share = g / min(rows, GROUPS);
+    const bool on = row < row0 + rows && share < deal;
+    JoinSum sum = {-INFINITY, 0.f, make_float4(0, 0, 0, 0)};
+    if (on) {
+      const int m_at = ROWS * HD + row, l_at = m_at + ROWS, o_at = row * HD + d;
+      if (share == 0) sum.add(first[m_at], first[l_at], *reinterpret_cast<const float4*>(first + o_at));
+      constexpr int U = 4;  // parts in flight
+      for (int k0 = share; k0 < n_after; k0 += U * deal) {
+        float mk[U], lk[U];
+        float4 ok[U];
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+          const int k = k0 + x * deal;
+          const bool has = k < n_after && holds[k];
+          const float* s = rest + 2 * SLOT * (has ? k : 0);
+          mk[x] = has ? s[m_at] : -INFINITY;
+          lk[x] = has ? s[l_at] : 0.f;
+          ok[x] = has ? *reinterpret_cast<const float4*>(s + o_at) : make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int x = 0; x < U; ++x) sum.add(mk[x], lk[x], ok[x]);
+      }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int r = cur.it.r0 + row, tok = cur.s.q0 + r / p.group, h = cur.kvh * p.group + r % p.group;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) +
-                                                (static_cast<long long>(tok) * p.heads + h) * p.out_hd + d);
-    *dst = Pair16<T>::pack(a0 * inv, a1 * inv);
+    if (deal > 1) {
+      sums[threadIdx.x] = sum;
+      __syncthreads();
+      if (on && share == 0)
+        for (int x = 1; x < deal; ++x) {
+          const JoinSum& y = sums[threadIdx.x + x * rows * TPR];
+          sum.add(y.m, y.l, y.o);
+        }
+    }
+    if (on && share == 0 && d < p.out_hd) {
+      const float inv = sum.l > 0.f ? 1.f / sum.l : 0.f;
+      const int r = cur.it.r0 + row, tok = cur.s.q0 + r / p.group, h = cur.kvh * p.group + r % p.group;
+      uint2* dst = reinterpret_cast<uint2*>(static_cast<T*>(p.out) +
+                                            (static_cast<long long>(tok) * p.heads + h) * p.out_hd + d);
+      *dst = make_uint2(Pair16<T>::pack(sum.o.x * inv, sum.o.y * inv), Pair16<T>::pack(sum.o.z * inv, sum.o.w * inv));
+    }
   }
 }
 
@@ -375,26 +466,24 @@ __device__ __forceinline__ uint32_t paged_rows_at(int r, int c) {
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
-    paged_rows_kernel(const PagedParams p, long long min_units) {
+    paged_rows_kernel(const PagedParams p, int tpi, int min_tiles) {
   using L = PagedRowsLayout<HD>;
   using PT = Pair16<T>;
-  constexpr int TK = L::TK, NST = L::NST, RPT = 16;
+  constexpr int TK = L::TK, NST = L::NST;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ PagedStart starts[L::WARPS];
+  __shared__ PagedCut cuts[L::WARPS + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = ((smem_u32(smem_raw) + 127) & ~127u) + warp * NST * L::STAGE;
-  long long total, per;
+  long long per;
   const int worker0 = blockIdx.x * L::WARPS;
-  paged_schedule<TK, L::WARPS, L::THREADS>(p, RPT, min_units, worker0, starts, &total, &per);
+  paged_schedule<TK, L::WARPS + 1, L::THREADS>(p, tpi, min_tiles, worker0, cuts, &per);
   paged_zero_outside(p, L::THREADS);
-  if (starts[warp].b < 0) return;
+  pdl_trigger();
   const int worker = worker0 + warp;
-  const long long begin = worker * per;
-  const int n_units = static_cast<int>(min(per, total - begin));
-
-  PagedCursor<TK> cur, ahead;
-  cur.seek(p, starts[warp].b, starts[warp].off, RPT);
+  PagedWalk<TK> cur, ahead;
+  if (!cur.begin(p, cuts[warp], cuts[warp + 1], tpi)) return;
   ahead = cur;
+  bool more = true;  // `ahead` has a tile
 
   // Copies the K and V tile under `ahead` into stage st and moves it on.
   auto fetch = [&](int st) {
@@ -418,12 +507,12 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
       cp_async_16(sv + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.v_pages) + at * p.v_stride + in_page,
                   ok ? 16u : 0u);
     }
-    if (++ahead.i == ahead.it.n) ahead.next_item(p, RPT);
+    if (++ahead.i == ahead.i1) more = ahead.next(p, tpi);
   };
 
-  int fetched = 0;
-  for (; fetched < NST - 1; ++fetched) {
-    if (fetched < n_units) fetch(fetched);
+#pragma unroll
+  for (int st = 0; st < NST - 1; ++st) {
+    if (more) fetch(st);
     cp_async_commit();
   }
 
@@ -432,9 +521,9 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
   float m[2], l[2];
   int pos[2];
   bool fresh = true;
-  const int seg0 = cur.i;       // the piece begins this far into its first item
-  bool from_start = seg0 == 0;  // the current item's first tile is in this piece
-  for (int u = 0; u < n_units; ++u) {
+  bool from_start = cur.i == 0;  // the current item's first tile is in this piece
+  int st = 0;
+  for (;;) {
     if (fresh) {
       fresh = false;
 #pragma unroll
@@ -454,12 +543,12 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
 #pragma unroll
       for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
     }
-    if (fetched < n_units) fetch(fetched % NST);
-    ++fetched;
+    if (more) fetch(st == 0 ? NST - 1 : st - 1);
     cp_async_commit();
     cp_async_wait<NST - 1>();
     __syncwarp();
-    const uint32_t sk = ring + u % NST * L::STAGE, sv = sk + L::TILE;
+    const uint32_t sk = ring + st * L::STAGE, sv = sk + L::TILE;
+    if (++st == NST) st = 0;
     const int k0 = cur.it.tile(cur.i) * TK;
     const bool whole = cur.it.whole(p, k0);
 
@@ -540,8 +629,8 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
     }
     __syncwarp();  // every lane has read the stage before a later round refills it
 
-    const bool last = cur.i + 1 == cur.it.n;
-    if (last || u + 1 == n_units) {
+    if (++cur.i == cur.i1) {  // the item, or its part in this piece, is done
+      const bool last = cur.i1 == cur.it.n;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(~0u, l[h], 1);
@@ -578,9 +667,7 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
       }
       fresh = true;
       from_start = true;
-      if (u + 1 < n_units) cur.next_item(p, RPT);
-    } else {
-      ++cur.i;
+      if (!cur.next(p, tpi)) break;
     }
   }
   cp_async_wait<0>();

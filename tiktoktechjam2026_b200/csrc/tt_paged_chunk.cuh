@@ -149,38 +149,17 @@ struct ChunkHalf {
   int last;        // the last tile of the segment that it sees, -1: none
 };
 
-// Walks a worker's piece segment by segment.
+// Walks a worker's piece; a segment is the part of one item that lies in it.
 template <int HD>
-struct ChunkWalk {
-  using L = PagedChunkLayout<HD>;
-  static constexpr int BN = L::BN;
-  PagedCursor<BN> cur;
-  int left;    // units of the piece from this segment on
-  int i0, i1;  // the segment's tiles
-  __device__ __forceinline__ void load() {
-    i0 = cur.i;
-    i1 = min(cur.it.n, i0 + left);
-  }
-  __device__ __forceinline__ void begin(const PagedParams& p, const PagedStart& s, int n_units, int rpt) {
-    cur.seek(p, s.b, s.off, rpt);
-    left = n_units;
-    load();
-  }
-  // The next segment; false at the end of the piece.
-  __device__ __forceinline__ bool next(const PagedParams& p, int rpt) {
-    left -= i1 - i0;
-    if (left <= 0) return false;
-    cur.next_item(p, rpt);
-    load();
-    return true;
-  }
+struct ChunkWalk : PagedWalk<PagedChunkLayout<HD>::BN> {
+  static constexpr int BN = PagedChunkLayout<HD>::BN;
   __device__ __forceinline__ ChunkHalf half(const PagedParams& p, int h, int half_tokens) const {
     ChunkHalf x;
     const int hr = half_tokens * p.group;
-    x.rows = min(max(cur.it.rows - h * hr, 0), hr);
+    x.rows = min(max(this->it.rows - h * hr, 0), hr);
     x.range = {0, 0, 0};
     x.last = -1;
-    x.p0 = cur.it.p0 + h * half_tokens;
+    x.p0 = this->it.p0 + h * half_tokens;
     x.p1 = x.p0 + (x.rows - 1) / p.group;
     if (x.rows == 0) return x;
     const int end = x.p1 < 0 ? 0 : x.p1 / BN + 1;  // one past the last tile a row sees
@@ -189,17 +168,17 @@ struct ChunkWalk {
     } else {
       const int from = max(x.p0 - p.window + 1, 0) / BN;  // first tile in the window
       const int sink = (min(p.sinks, BN * end) + BN - 1) / BN;
-      if (cur.it.n_sink == cur.it.n) {  // no gap: the index is the tile
+      if (this->it.n_sink == this->it.n) {  // no gap: the index is the tile
         x.range.a = min(sink, end);
         x.range.c = max(from, x.range.a);
         x.range.e = end;
       } else {
-        x.range.a = min(cur.it.n_sink, end);
-        x.range.c = max(from - cur.it.w_tile, 0) + cur.it.n_sink;
-        x.range.e = end - cur.it.w_tile + cur.it.n_sink;
+        x.range.a = min(this->it.n_sink, end);
+        x.range.c = max(from - this->it.w_tile, 0) + this->it.n_sink;
+        x.range.e = end - this->it.w_tile + this->it.n_sink;
       }
     }
-    x.last = x.range.last(i0, i1);
+    x.last = x.range.last(this->i, this->i1);
     return x;
   }
 };
@@ -212,19 +191,21 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                        const __grid_constant__ CUtensorMap tmV, const PagedParams p, int half_tokens,
-                       long long min_units) {
+                       int min_tiles) {
   using L = PagedChunkLayout<HD>;
   using PT = Pair16<T>;
   constexpr int BN = L::BN, NT = L::NT, NSB = L::NSB, NST = L::NST, NQ = L::NQ, NOB = L::NOB;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ PagedStart start;
+  __shared__ PagedCut cuts[2];
   __shared__ ChunkWalk<HD> saved[6 * NT];  // walks at rest: the softmax warps', then two of each MMA warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int half_rows = half_tokens * p.group, rpt = NT * half_rows;
-  long long total, per;
-  paged_schedule<BN, 1, L::THREADS>(p, rpt, min_units, blockIdx.x, &start, &total, &per);
+  const int half_rows = half_tokens * p.group, tpi = NT * half_tokens;
+  long long per;
+  paged_schedule<BN, 2, L::THREADS>(p, tpi, min_tiles, blockIdx.x, cuts, &per);
   paged_zero_outside(p, L::THREADS);
-  if (start.b < 0) return;
+  pdl_trigger();
+  ChunkWalk<HD> walk;
+  if (!walk.begin(p, cuts[0], cuts[1], tpi)) return;
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -263,9 +244,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const Watchdog wd{p.err, abort_flag, p.timeout_ns};
-  const int n_units = static_cast<int>(min(per, total - blockIdx.x * per));
   const int page_rows = 1 << p.page_shift;
-  ChunkWalk<HD> walk;
 
   if (warp == L::W_PROD) {
     // -------------------------------------------------------------- producer
@@ -279,7 +258,6 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     int u = 0, st = 0, nq[NT] = {};
     uint32_t ph = 0;
     bool ok = true;
-    walk.begin(p, start, n_units, rpt);
     do {
 #pragma unroll
       for (int h = 0; h < NT; ++h) {
@@ -289,29 +267,29 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         if (lane == 0) ok = wait_phase(&b[L::H_QE + qb], ((nq[h] / NQ) & 1) ^ 1, wd, 0x531);
         if (!(ok = __shfl_sync(~0u, ok, 0))) break;
         if (lane == 0) {
-          const int tok = walk.cur.s.q0 + walk.cur.it.r0 / p.group + h * half_tokens;
+          const int tok = walk.s.q0 + walk.it.r0 / p.group + h * half_tokens;
           mbar_arrive_expect_tx(&b[L::H_QF + qb], L::NATOM * half_rows * L::ROW);
 #pragma unroll
           for (int a = 0; a < L::NATOM; ++a)
             tma_load_3d(smem + L::OFF_Q + (h * NQ + qb) * L::Q_BYTES + a * L::Q_ATOM, &tmQ, &b[L::H_QF + qb],
-                        a * L::ATOM, walk.cur.kvh * p.group, tok);
+                        a * L::ATOM, walk.kvh * p.group, tok);
         }
         ++nq[h];
       }
       if (!ok) break;
-      const int* row = p.tables + walk.cur.s.slot * p.table_stride;
-      const int n_keys = walk.cur.s.L;
+      const int* row = p.tables + walk.s.slot * p.table_stride;
+      const int n_keys = walk.s.L;
       // The page of this lane's box of tile i (n_pages, past the end, where there is none).
       auto page_of = [&](int i) -> int {
-        const int key = walk.cur.it.tile(i) * BN + lane * box;
+        const int key = walk.it.tile(i) * BN + lane * box;
         int pg = -1;
         if (lane < n_box && key < n_keys) pg = row[key >> p.page_shift];
         return pg < 0 || pg >= p.n_pages ? p.n_pages : pg;
       };
-      int page = page_of(walk.i0);
-      for (int i = walk.i0; i < walk.i1; ++i, ++u) {
+      int page = page_of(walk.i);
+      for (int i = walk.i; i < walk.i1; ++i, ++u) {
         const int next = i + 1 < walk.i1 ? page_of(i + 1) : 0;  // a tile ahead: its latency is off the path
-        const int at = walk.cur.kvh * page_rows + ((walk.cur.it.tile(i) * BN + lane * box) & (page_rows - 1));
+        const int at = walk.kvh * page_rows + ((walk.it.tile(i) * BN + lane * box) & (page_rows - 1));
         if (lane == 0) {
           ok = wait_phase(&bars[L::B_E + st], ph ^ 1, wd, 0x532);
           if (ok) mbar_arrive_expect_tx(&bars[L::B_F + st], 2 * L::KV_BYTES);
@@ -333,7 +311,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         if (!ok) break;
         page = next;
       }
-    } while (ok && walk.next(p, rpt));
+    } while (ok && walk.next(p, tpi));
     // Let every copy this warp started land before the CTA may exit.
     if (lane == 0) {
       for (int h = 0; h < NT; ++h)
@@ -347,13 +325,12 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     int st = 0;
     uint32_t ph = 0;
     bool ok = true;
-    walk.begin(p, start, n_units, rpt);
     do {
       // Only the item's last tile can hold the end of the sequence.
-      const int r0 = walk.cur.s.L - walk.cur.it.tile(walk.cur.it.n - 1) * BN;
+      const int r0 = walk.s.L - walk.it.tile(walk.it.n - 1) * BN;
       const int r1 = min((r0 + page_rows - 1) & ~(page_rows - 1), BN);  // the end of its page, or of the tile
-      const int fix_at = r0 > 0 && r0 < BN && (r0 & (page_rows - 1)) != 0 ? walk.cur.it.n - 1 : -1;
-      for (int i = walk.i0; i < walk.i1; ++i) {
+      const int fix_at = r0 > 0 && r0 < BN && (r0 & (page_rows - 1)) != 0 ? walk.it.n - 1 : -1;
+      for (int i = walk.i; i < walk.i1; ++i) {
         if (!(ok = warp_wait_phase(&bars[L::B_F + st], ph, wd, 0x534))) break;
         if (i == fix_at) {
           const uint32_t base = smem_u32(smem + L::OFF_V + st * L::KV_BYTES);
@@ -370,7 +347,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
           ph ^= 1;
         }
       }
-    } while (ok && walk.next(p, rpt));
+    } while (ok && walk.next(p, tpi));
   } else if (warp >= L::W_MMA && warp < L::W_MMA + NT) {
     // -------------------------------------------------------------- MMA issuer of a half
     // The warp's own instructions are on the critical path.  It walks the loop
@@ -398,15 +375,15 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     };
     auto read = [&](const ChunkWalk<HD>& w) -> Segment {
       const ChunkHalf x = w.half(p, h, half_tokens);
-      const int r0 = w.cur.s.L - w.cur.it.tile(w.cur.it.n - 1) * BN;
-      const int fix = r0 > 0 && r0 < BN && (r0 & (page_rows - 1)) != 0 ? w.cur.it.n - 1 : -1;
-      return {__shfl_sync(~0u, w.i0, 0),      __shfl_sync(~0u, w.i1, 0),      __shfl_sync(~0u, x.range.a, 0),
+      const int r0 = w.s.L - w.it.tile(w.it.n - 1) * BN;
+      const int fix = r0 > 0 && r0 < BN && (r0 & (page_rows - 1)) != 0 ? w.it.n - 1 : -1;
+      return {__shfl_sync(~0u, w.i, 0),       __shfl_sync(~0u, w.i1, 0),      __shfl_sync(~0u, x.range.a, 0),
               __shfl_sync(~0u, x.range.c, 0), __shfl_sync(~0u, x.range.e, 0), __shfl_sync(~0u, x.last, 0),
               __shfl_sync(~0u, fix, 0)};
     };
     if (lane == 0) {
-      walks[0].begin(p, start, n_units, rpt);
-      walks[1] = walks[0];
+      walks[0] = walk;
+      walks[1] = walk;
     }
     __syncwarp();
     Segment ss = read(walks[0]);
@@ -417,7 +394,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     auto step_s = [&]() -> bool {
       if (ss.i == ss.i1) {
         if (!more_s) return true;
-        more_s = __shfl_sync(~0u, lane == 0 ? walks[0].next(p, rpt) : false, 0);
+        more_s = __shfl_sync(~0u, lane == 0 ? walks[0].next(p, tpi) : false, 0);
         __syncwarp();
         if (!more_s) return true;
         ss = read(walks[0]);
@@ -503,7 +480,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         if (++v_st == NST) v_st = 0;
         if (!(ok = step_s())) break;
       }
-      more = ok && __shfl_sync(~0u, lane == 0 ? walks[1].next(p, rpt) : false, 0);
+      more = ok && __shfl_sync(~0u, lane == 0 ? walks[1].next(p, tpi) : false, 0);
       __syncwarp();
     }
     // All MMAs the elected lane issued must finish before TMEM is released.
@@ -579,10 +556,10 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
 
     // The walk rests in shared memory while a segment is worked on: its
     // registers would push the scores out.
-    if (lane == 0) saved[warp].begin(p, start, n_units, rpt);
+    if (lane == 0) saved[warp] = walk;
     bool more = true;
     int units = 0;  // of the segments so far
-    for (; ok && more; more = __shfl_sync(~0u, lane == 0 ? saved[warp].next(p, rpt) : false, 0)) {
+    for (; ok && more; more = __shfl_sync(~0u, lane == 0 ? saved[warp].next(p, tpi) : false, 0)) {
       ChunkRange range;
       int i, last, p0, p1, pos, n_sink, w_shift, unit;  // unit: ring position of tile i
       bool on;
@@ -594,21 +571,21 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         const ChunkWalk<HD>& w = saved[warp];
         const ChunkHalf x = w.half(p, h, half_tokens);
         range = x.range;
-        i = w.i0 < range.a ? w.i0 : max(range.c, w.i0);
+        i = w.i < range.a ? w.i : max(range.c, w.i);
         last = x.last;
-        unit = units + i - w.i0;
-        units += w.i1 - w.i0;
+        unit = units + i - w.i;
+        units += w.i1 - w.i;
         p0 = x.p0;
         p1 = x.p1;
         pos = x.p0 + row / p.group;
         on = row < x.rows;
-        n_sink = w.cur.it.n_sink;
-        w_shift = w.cur.it.w_tile - n_sink;
-        const int r = w.cur.it.r0 + item_row;
-        const long long tok = w.cur.s.q0 + r / p.group;
-        if (on) out = static_cast<T*>(p.out) + (tok * p.heads + w.cur.kvh * p.group + r % p.group) * p.out_hd;
-        if (w.i0 > 0 || w.i1 < w.cur.it.n)
-          part = p.part + (2ll * blockIdx.x + (w.i0 > 0 ? 0 : 1)) * paged_slot_floats<L::ROWS, HD>();
+        n_sink = w.it.n_sink;
+        w_shift = w.it.w_tile - n_sink;
+        const int r = w.it.r0 + item_row;
+        const long long tok = w.s.q0 + r / p.group;
+        if (on) out = static_cast<T*>(p.out) + (tok * p.heads + w.kvh * p.group + r % p.group) * p.out_hd;
+        if (w.i > 0 || w.i1 < w.it.n)
+          part = p.part + (2ll * blockIdx.x + (w.i > 0 ? 0 : 1)) * paged_slot_floats<L::ROWS, HD>();
       }
       __syncwarp();  // read before lane 0 moves it on
       if (last < 0) {  // nothing here for this half
