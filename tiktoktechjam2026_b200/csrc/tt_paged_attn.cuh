@@ -114,26 +114,47 @@ __device__ __forceinline__ int paged_q_tiles(const PagedParams& p, const PagedSe
   return rows >= p.row_lo && rows <= p.row_hi ? (s.T + tpi - 1) / tpi : 0;
 }
 
-// sum over j < n of max(a + j d, 0), d > 0.
-__device__ __forceinline__ long long ramp_sum(long long a, int d, int n) {
-  const int j0 = a >= 0 ? 0 : static_cast<int>(min((-a + d - 1) / d, static_cast<long long>(n)));
-  const long long m = n - j0;
+// a / b for a >= 0, b > 0; 64-bit division is a long subroutine and rarely needed.
+__device__ __forceinline__ long long div_pos(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
+// sum over j < n of max(a + j d, 0), d > 0, where j0 is the first j with a + j d >= 0.
+__device__ __forceinline__ long long ramp_sum(long long a, int d, int j0, int n) {
+  const long long m = max(n - j0, 0);
   return m * (a + static_cast<long long>(j0) * d) + d * (m * (m - 1) / 2);
+}
+__device__ __forceinline__ int ramp_start(long long a, int d) {
+  return a >= 0 ? 0 : static_cast<int>(div_pos(-a + d - 1, d));
 }
 
 // Length on the line of the first q of sequence s's nq items for one KV head:
 // item j spans the keys up to position p1(j), less, under a window, those
 // between the first tokens and the window of p0(j).
 template <int TK>
-__device__ __forceinline__ long long paged_line(const PagedParams& p, const PagedSeq& s, int q, int nq, int tpi) {
-  if (q == 0) return 0;
-  const long long base = s.L - s.T;
-  const int whole = q == nq ? q - 1 : q;  // the last item may hold fewer tokens
-  long long len = static_cast<long long>(q) * (kPagedItemTiles * TK) + ramp_sum(base + tpi, tpi, whole);
-  if (q == nq) len += s.L;
-  if (p.window > 0) len -= ramp_sum(base - p.window + 1 - p.sinks, tpi, q);
-  return len;
-}
+struct PagedLine {
+  long long up, gap;  // p1(0) + 1; p0(0) + 1 - window - sinks
+  int up0, gap0, nq, tpi, L;
+  bool window;
+  __device__ __forceinline__ PagedLine(const PagedParams& p, const PagedSeq& s, int nq_, int tpi_)
+      : nq(nq_), tpi(tpi_), L(s.L), window(p.window > 0) {
+    const long long base = s.L - s.T;
+    up = base + tpi;
+    up0 = ramp_start(up, tpi);
+    gap = base - p.window + 1 - p.sinks;
+    gap0 = window ? ramp_start(gap, tpi) : 0;
+  }
+  __device__ __forceinline__ long long before(int q) const {
+    if (q == 0) return 0;
+    const int whole = q == nq ? q - 1 : q;  // the last item may hold fewer tokens
+    long long len = static_cast<long long>(q) * (kPagedItemTiles * TK) + ramp_sum(up, tpi, up0, whole);
+    if (q == nq) len += L;
+    if (window) len -= ramp_sum(gap, tpi, gap0, q);
+    return len;
+  }
+  __device__ __forceinline__ long long all() const { return before(nq); }
+};
 
 // A cut of the line: sequence and length into it (b < 0: the end of the line).
 struct PagedCut {
@@ -148,21 +169,21 @@ struct PagedWalk {
   PagedSeq s;
   PagedItem<TK> it;
   int end_b, end_kvh, end_qt, end_i;
-  long long start, len;  // seek: the line before the item within (sequence, KV head), and the item's length
+  long long at, len;  // seek: where in the item the cut falls, and the item's length
 
   __device__ __forceinline__ void seek(const PagedParams& p, const PagedCut& c, int tpi) {
     b = c.b;
     s = paged_seq(p, b);
     nq = paged_q_tiles(p, s, tpi);
-    const long long head = paged_line<TK>(p, s, nq, nq, tpi);
-    kvh = static_cast<int>(c.off / head);
+    const PagedLine<TK> line(p, s, nq, tpi);
+    const long long head = line.all();
+    kvh = static_cast<int>(div_pos(c.off, head));
     const long long off = c.off - kvh * head;
     int lo = 0, hi = nq;  // the last item that begins at or before off
-    start = 0;
-    long long next = head;
+    long long start = 0, next = head;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      const long long x = paged_line<TK>(p, s, mid, nq, tpi);
+      const long long x = line.before(mid);
       if (x <= off) {
         lo = mid;
         start = x;
@@ -172,12 +193,17 @@ struct PagedWalk {
       }
     }
     qt = lo;
+    at = off - start;
     len = next - start;
     it.set(p, s, qt, tpi);
-    i = tile_at(off - start);
+    i = tile_at(at);
   }
-  // The tile on which a cut at length x of the item falls.
-  __device__ __forceinline__ int tile_at(long long x) const { return static_cast<int>(x * it.n / len); }
+  // The tile on which a cut at length x of the item falls.  Every kernel and
+  // worker must find the same one: one multiplication and no contraction.
+  __device__ __forceinline__ int tile_at(long long x) const {
+    return min(static_cast<int>(__fmul_rn(__ll2float_rn(x), __fdiv_rn(__int2float_rn(it.n), __ll2float_rn(len)))),
+               it.n - 1);
+  }
 
   __device__ __forceinline__ bool at_end() const { return b == end_b && kvh == end_kvh && qt == end_qt; }
   // Whether the piece from cut c to cut e holds any tile; places the walk on its first.
@@ -228,7 +254,7 @@ __device__ __forceinline__ void paged_schedule(const PagedParams& p, int tpi, in
     if (b >= p.batch) return 0;
     const PagedSeq s = paged_seq(p, b);
     const int nq = paged_q_tiles(p, s, tpi);
-    return paged_line<TK>(p, s, nq, nq, tpi) * p.kv_heads;
+    return nq == 0 ? 0 : PagedLine<TK>(p, s, nq, tpi).all() * p.kv_heads;
   };
   const long long mine = length(tid);  // kept for the scan below: most batches are one round
   long long sum = mine;
@@ -240,7 +266,7 @@ __device__ __forceinline__ void paged_schedule(const PagedParams& p, int tpi, in
   __syncthreads();
   long long all = 0;
   for (int w = 0; w < NWARPS; ++w) all += warp_sum[w];
-  const long long each = max((all + p.n_workers - 1) / p.n_workers, static_cast<long long>(min_tiles) * TK);
+  const long long each = max(div_pos(all + p.n_workers - 1, p.n_workers), static_cast<long long>(min_tiles) * TK);
   *per = each;
   long long carry = 0;
   for (int b0 = 0; b0 < p.batch && all > 0; b0 += THREADS) {
@@ -361,25 +387,28 @@ struct JoinSum {
 
 template <typename T, int HD, int TK, int ROWS, int RB>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedParams p, int tpi, int min_tiles) {
-  __shared__ PagedCut cuts[2];
+  __shared__ PagedCut cut;
   __shared__ uint8_t holds[kPagedMaxWorkers];  // whether the k-th worker from c on has a part
   __shared__ JoinSum sums[kJoinThreads];
+  __shared__ PagedWalk<TK> cur;
+  __shared__ int n_after;  // workers from c on that start inside the item; 0: nothing to join here
   long long per;
   const int c = blockIdx.x + 1;  // worker 0 starts at an item's beginning
-  paged_schedule<TK, 2, kJoinThreads>(p, tpi, min_tiles, c - 1, cuts, &per);
-  if (cuts[1].b < 0) return;
-  PagedWalk<TK> cur;
-  cur.seek(p, cuts[1], tpi);
-  const int row0 = blockIdx.y * RB, rows = min(cur.it.rows - row0, RB);
-  if (cur.i == 0 || rows <= 0) return;
-  // Length into the item at which worker c starts; the others lie `per` apart.
-  const long long at = cuts[1].off - cur.kvh * paged_line<TK>(p, cur.s, cur.nq, cur.nq, tpi) - cur.start;
-  if (at > per && cur.tile_at(at - per) > 0) return;  // worker c - 1 starts inside too
-  const int n_after = static_cast<int>((cur.len - at + per - 1) / per);  // workers c .. that start inside
+  paged_schedule<TK, 1, kJoinThreads>(p, tpi, min_tiles, c, &cut, &per);
+  if (cut.b < 0) return;
+  if (threadIdx.x == 0) {
+    cur.seek(p, cut, tpi);
+    const bool mine = cur.i > 0 && cur.it.rows > static_cast<int>(blockIdx.y) * RB &&
+                      !(cur.at > per && cur.tile_at(cur.at - per) > 0);  // worker c - 1 starts inside too
+    n_after = mine ? static_cast<int>(div_pos(cur.len - cur.at + per - 1, per)) : 0;
+  }
+  __syncthreads();
+  if (n_after == 0) return;
   for (int k = threadIdx.x; k < n_after; k += kJoinThreads)
-    holds[k] = cur.tile_at(at + k * per) < (k + 1 < n_after ? cur.tile_at(at + (k + 1) * per) : cur.it.n);
+    holds[k] = cur.tile_at(cur.at + k * per) < (k + 1 < n_after ? cur.tile_at(cur.at + (k + 1) * per) : cur.it.n);
   __syncthreads();
   pdl_wait();
+  const int row0 = blockIdx.y * RB, rows = min(cur.it.rows - row0, RB);
   constexpr long long SLOT = paged_slot_floats<ROWS, HD>();
   const float* first = p.part + (2ll * (c - 1) + 1) * SLOT;
   const float* rest = p.part + 2ll * c * SLOT;  // then every 2 SLOT

@@ -204,8 +204,11 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   paged_schedule<BN, 2, L::THREADS>(p, tpi, min_tiles, blockIdx.x, cuts, &per);
   paged_zero_outside(p, L::THREADS);
   pdl_trigger();
-  ChunkWalk<HD> walk;
-  if (!walk.begin(p, cuts[0], cuts[1], tpi)) return;
+  __shared__ bool any;
+  if (threadIdx.x == 0) any = saved[0].begin(p, cuts[0], cuts[1], tpi);
+  __syncthreads();
+  if (!any) return;
+  ChunkWalk<HD> walk = saved[0];
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
