@@ -221,10 +221,12 @@ int tt_cache_reserve(const tt_kv_cache* cache, const int* cu_q, const int* slots
 /* Writes K and V of the new tokens (already counted by lens) into one layer's
  * pages.  k and v are [n_tokens, kv_heads, head_dim] with element strides
  * {token, head, feature}: dense in the features (16-byte aligned rows), or
- * dense in the tokens (tt_qkv_projection's vt). */
+ * dense in the tokens (tt_qkv_projection's vt).  status (device, or NULL): the
+ * status of the tt_cache_reserve that made the room; nothing is written where
+ * it is not 0. */
 int tt_cache_append(const tt_kv_cache* cache, const void* k, const int64_t* k_strides, const void* v,
                     const int64_t* v_strides, int n_tokens, const int* cu_q, const int* slots,
-                    int batch, void* stream);
+                    int batch, const int* status, void* stream);
 
 /* Releases pages of n slots (all n_slots when slots is NULL): every page, the
  * length becoming 0 (window 0), or with a window those pages that no later

@@ -132,7 +132,7 @@ SIGNATURES = {
     "tt_cache_append": (
         c_int,
         [POINTER(KVCache), c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_int, c_void_p, c_void_p, c_int,
-         c_void_p],
+         c_void_p, c_void_p],
     ),
     "tt_cache_release": (c_int, [POINTER(KVCache), c_void_p, c_int, c_int, c_int, c_void_p]),
     "tt_cache_fork": (c_int, [POINTER(KVCache), c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),

@@ -203,7 +203,8 @@ __device__ __forceinline__ void append_one(const CacheParams& c, const AppendSrc
 
 __global__ void __launch_bounds__(kAppendThreads)
     cache_append_kernel(const CacheParams c, const AppendSrc k, const AppendSrc v, const int* cu_q, const int* slots,
-                        int batch, int n_tokens) {
+                        int batch, int n_tokens, const int* status) {
+  if (status && *status != 0) return;  // no room was made: the lengths do not count these tokens
   extern __shared__ uint16_t tile[];
   __shared__ int dst_page[kAppendTokens], dst_row[kAppendTokens];
   const int t0 = blockIdx.x * kAppendTokens, h = blockIdx.y, hd = c.row_bytes / 2;

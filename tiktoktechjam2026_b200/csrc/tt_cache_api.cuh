@@ -198,7 +198,7 @@ int tt_cache_reserve(const tt_kv_cache* cache, const int* cu_q, const int* slots
 
 int tt_cache_append(const tt_kv_cache* cache, const void* k, const int64_t* k_strides, const void* v,
                     const int64_t* v_strides, int n_tokens, const int* cu_q, const int* slots, int batch,
-                    void* stream) {
+                    const int* status, void* stream) {
   return guarded([&]() -> int {
     DeviceState* ds;
     if (int rc = current_device_state(&ds)) return rc;
@@ -224,7 +224,7 @@ int tt_cache_append(const tt_kv_cache* cache, const void* k, const int64_t* k_st
     if (int rc = prepare_kernel(cache_append_kernel, smem)) return rc;
     launch_kernel(cache_append_kernel, dim3((n_tokens + kAppendTokens - 1) / kAppendTokens, c.kv_heads),
                   kAppendThreads, smem, static_cast<cudaStream_t>(stream), c, src[0], src[1], cu_q, slots, batch,
-                  n_tokens);
+                  n_tokens, status);
     return after_launch("cache append");
   });
 }

@@ -21,7 +21,8 @@ from typing import Dict, Optional, Sequence
 import torch
 import torch.nn as nn
 
-from . import _lib
+from . import _lib, ops
+from .kv_cache import PagedKVCache
 
 
 @dataclass(frozen=True)
@@ -484,6 +485,80 @@ class B200Transformer(nn.Module):
             stream.synchronize()
         return out
 
+
+    def extend(
+        self,
+        x: torch.Tensor,
+        cache: "PagedKVCache",
+        cu_q: Optional[torch.Tensor] = None,
+        slots: Optional[torch.Tensor] = None,
+        *,
+        window: int = 0,
+        sinks: int = 0,
+        max_q_len: Optional[int] = None,
+        check: bool = True,
+    ) -> torch.Tensor:
+        """The rows ``forward`` would give for new tokens at the end of cached sequences.
+
+        ``x`` holds the new tokens, FP32: [B, T, d_model], T for each sequence, or packed
+        [N, d_model] with ``cu_q`` (int32 [B + 1], rows cu_q[b] .. cu_q[b + 1] - 1 are sequence b's).
+        ``slots`` (int32 [B], distinct; 0 .. B - 1 without it) names the cache slots they extend.
+        Makes room, writes K and V of every layer and attends over the pages, so a prompt can come in
+        chunks of any length and answers token by token.  With ``window`` a token sees the last
+        ``window`` ones, itself included, and the first ``sinks``.  ``check`` waits for the
+        reservation and raises if the cache has no room; without it nothing waits, a refused call
+        leaves the cache as it was and its result is meaningless (``cache.check()`` tells).
+        """
+        cfg = self.config
+        if not cfg.causal:
+            raise ValueError("extend needs a causal model: earlier rows do not depend on later tokens")
+        if x.dtype != torch.float32 or not x.is_cuda or x.shape[-1] != cfg.d_model:
+            raise ValueError(f"extend takes FP32 CUDA tokens [B, T, {cfg.d_model}] or [N, {cfg.d_model}]")
+        if (cu_q is None) != (x.dim() == 3) or x.dim() not in (2, 3):
+            raise ValueError("pass [B, T, d_model] tokens, or [N, d_model] tokens with cu_q")
+        if cache.device != x.device:
+            raise ValueError(f"the cache is on {cache.device}, x on {x.device}")
+        if cache.k.shape[0] != cfg.num_layers or cache.k.shape[2] != cfg.num_heads or (
+                cache.head_dim != cfg.d_model // cfg.num_heads) or cache.k.dtype != torch.float16:
+            raise ValueError("the cache does not have this model's layers, heads and FP16 pages")
+        if cu_q is None:
+            batch, steps = x.shape[:2]
+            max_q_len = steps
+            cu_q = torch.arange(0, batch * steps + 1, max(steps, 1), dtype=torch.int32, device=x.device)[: batch + 1]
+            if steps == 0:
+                cu_q = torch.zeros(batch + 1, dtype=torch.int32, device=x.device)
+        rows = x.reshape(-1, cfg.d_model).contiguous()
+        n = rows.shape[0]
+        cache.reserve(cu_q, slots)
+        if check:
+            cache.check()
+        if n == 0:
+            return torch.empty_like(x)
+        eps, last = float(self.layers[0].norm1.eps), cfg.num_layers - 1
+        norm = ops.layernorm_rows(rows, self.layers[0].norm1.weight, self.layers[0].norm1.bias, eps)
+        for i, layer in enumerate(self.layers):
+            att, nxt = layer.attention, self.final_norm if i == last else self.layers[i + 1].norm1
+
+            def bias(name: str, linear: nn.Linear) -> torch.Tensor:
+                return self._bias_fp32.get(f"layers.{i}.{name}", linear.bias)
+
+            q, k, vt = ops.qkv_projection(norm.view(1, n, -1), att.qkv_proj.weight, bias("attention.qkv_proj", att.qkv_proj),
+                                          cfg.num_heads)
+            cache.append(i, k[0].transpose(0, 1), vt[0, :, :, :n].permute(2, 0, 1), cu_q, slots)
+            ctx = cache.attend(i, q[0].transpose(0, 1), cu_q, slots, scale=att.scale, window=window, sinks=sinks,
+                               max_q_len=max_q_len)
+            rows, norm = ops.linear_residual_layernorm(ctx, att.out_proj.weight, bias("attention.out_proj", att.out_proj), rows,
+                                                       layer.norm2.weight, layer.norm2.bias, eps)
+            out_type = torch.float32 if i == last else torch.float16
+            b_in, b_out = bias("ffn_in", layer.ffn_in), bias("ffn_out", layer.ffn_out)
+            if cfg.d_model in (32, 64, 128, 256) and cfg.ffn_dim % 128 == 0:
+                rows, norm = ops.ffn_residual_layernorm(norm, layer.ffn_in.weight, b_in, layer.ffn_out.weight, b_out, rows,
+                                                        nxt.weight, nxt.bias, eps, out_type)
+            else:
+                hidden = ops.linear_gelu(norm, layer.ffn_in.weight, b_in)
+                rows, norm = ops.linear_residual_layernorm(hidden, layer.ffn_out.weight, b_out, rows, nxt.weight, nxt.bias,
+                                                           eps, out_type)
+        return norm.view(x.shape)
 
     def capture_graph(self, x: torch.Tensor, valid_token_mask: Optional[torch.Tensor] = None) -> "GraphedForward":
         """Captures one forward over ``x`` as a CUDA graph (``tt_model_graph_create``).

@@ -188,55 +188,63 @@ def ffn_residual_layernorm(a: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, 
 # rows cu_q[b] .. cu_q[b + 1] - 1 of the token tensors.  ``PagedKVCache`` keeps
 # these tensors together.
 # ---------------------------------------------------------------------------
-_PAGED_DTYPES = (torch.float16, torch.bfloat16)
+PAGED_DTYPES = (torch.float16, torch.bfloat16)
 PAGE_SIZES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (8, 16, 32, 64, 128, 256)
 
 
-def _index(t: Optional[torch.Tensor], name: str, device: torch.device, dims: int = 1) -> int:
+def _index(t: Optional[torch.Tensor], name: str, device: int, dims: int = 1) -> int:
     """Address of an int32 index tensor (0 for None)."""
     if t is None:
         return 0
-    _need(t.dtype == torch.int32 and t.dim() == dims and t.device == device,
-          f"{name} must be an int32 tensor of {dims} dimension(s) on {device}")
-    _need(t.is_contiguous() if dims == 1 else t.stride(-1) == 1, f"{name} must be contiguous")
+    if t.dtype is not torch.int32 or t.get_device() != device or t.dim() != dims or (
+            t.stride(1) != 1 if dims == 2 else not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on cuda:{device}")
     return t.data_ptr()
 
 
 def _cache(k: Optional[torch.Tensor], v: Optional[torch.Tensor], tables: torch.Tensor, lens: torch.Tensor,
            refs: Optional[torch.Tensor], page: int = 0) -> KVCache:
-    dev = tables.device
-    _need(tables.is_cuda, "tables must be a CUDA tensor")
-    c = KVCache()
-    c.tables, c.lens, c.refs = _index(tables, "tables", dev, 2), _index(lens, "lens", dev), _index(refs, "refs", dev)
-    c.n_slots, c.table_width = tables.shape
-    c.table_stride = tables.stride(0)
-    _need(lens.shape[0] == c.n_slots, f"lens has {lens.shape[0]} entries, tables {c.n_slots} rows")
+    """struct tt_kv_cache of checked tensors.  (Messages are built on failure only: a decode step makes this call for
+    every layer.)"""
+    if not tables.is_cuda:
+        raise ValueError("tables must be a CUDA tensor")
+    dev = tables.get_device()
+    tables_at, lens_at, refs_at = _index(tables, "tables", dev, 2), _index(lens, "lens", dev), _index(refs, "refs", dev)
+    slots, width = tables.shape
+    if lens.shape[0] != slots:
+        raise ValueError(f"lens has {lens.shape[0]} entries, tables {slots} rows")
     if k is None:
-        c.page, c.n_pages = page, refs.shape[0]
-        return c
-    _need(k.dim() in (4, 5) and k.shape == v.shape, "k and v must be [pages, kv_heads, page, head_dim] pages of one "
-          "layer, or [layers, pages, ...], of one shape")
-    _need(k.dtype in _PAGED_DTYPES and v.dtype == k.dtype, "k and v pages must be FP16 or BF16")
-    _need(k.device == dev and v.device == dev, f"k and v pages must be on {dev}")
-    pages, c.kv_heads, c.page, c.head_dim = k.shape[-4:]
-    for t, name in ((k, "k"), (v, "v")):
-        st = t.stride()
-        _need(st[-1] == 1 and st[-2] == c.head_dim and st[-3] == c.page * c.head_dim,
-              f"each page of {name} must be contiguous")
-    c.k, c.v = k.data_ptr(), v.data_ptr()
-    c.k_page_stride, c.v_page_stride = k.stride(-4), v.stride(-4)
-    c.layers = 1
-    if k.dim() == 5:
-        c.layers, c.k_layer_stride, c.v_layer_stride = k.shape[0], k.stride(0), v.stride(0)
-    c.n_pages = pages
-    _need(refs is None or refs.shape[0] == pages, f"refs must have one entry for each of the {pages} pages")
-    return c
+        return KVCache(None, None, 0, 0, 0, 0, tables_at, tables.stride(0), lens_at, refs_at, 0, refs.shape[0], 0, page, 0,
+                       slots, width)
+    shape = k.shape
+    dims = len(shape)
+    if dims not in (4, 5) or v.shape != shape:
+        raise ValueError("k and v must be [pages, kv_heads, page, head_dim] pages of one layer, or [layers, pages, ...], "
+                         "of one shape")
+    if k.dtype not in PAGED_DTYPES or v.dtype is not k.dtype:
+        raise ValueError("k and v pages must be FP16 or BF16")
+    if k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"k and v pages must be on cuda:{dev}")
+    layers, k_layer, v_layer = 1, 0, 0
+    ks, vs = k.stride(), v.stride()
+    if dims == 5:
+        layers, k_layer, v_layer = shape[0], ks[0], vs[0]
+        shape, ks, vs = shape[1:], ks[1:], vs[1:]
+    pages, kv_heads, page, head_dim = shape
+    dense = (page * head_dim, head_dim, 1)
+    if ks[1:] != dense or vs[1:] != dense:
+        raise ValueError("each page of k and v must be contiguous")
+    if refs is not None and refs.shape[0] != pages:
+        raise ValueError(f"refs must have one entry for each of the {pages} pages")
+    return KVCache(k.data_ptr(), v.data_ptr(), k_layer, v_layer, ks[0], vs[0], tables_at, tables.stride(0), lens_at, refs_at,
+                   layers, pages, kv_heads, page, head_dim, slots, width)
 
 
-def _run(device: torch.device, fn, *args) -> None:
+def _run(device: int, fn, *args) -> None:
     """Calls a libtt_b200 entry point on the device's current stream."""
     stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
+    if torch.cuda.current_device() == device:
         check(fn(*args, stream))
         return
     with torch.cuda.device(device):
@@ -245,13 +253,15 @@ def _run(device: torch.device, fn, *args) -> None:
 
 def _batch(cu_q: torch.Tensor, slots: Optional[torch.Tensor], tables: torch.Tensor) -> Tuple[int, int, int]:
     """(address of cu_q, address of slots, sequences of the call)."""
-    n = cu_q.shape[0] - 1
-    _need(n >= 0, "cu_q needs at least one entry")
+    n, dev = cu_q.shape[0] - 1, tables.get_device()
+    if n < 0:
+        raise ValueError("cu_q needs at least one entry")
     if slots is None:
-        _need(n <= tables.shape[0], f"{n} sequences, but {tables.shape[0]} table rows")
-    else:
-        _need(slots.shape[0] == n, f"cu_q describes {n} sequences, slots {slots.shape[0]}")
-    return _index(cu_q, "cu_q", tables.device), _index(slots, "slots", tables.device), n
+        if n > tables.shape[0]:
+            raise ValueError(f"{n} sequences, but {tables.shape[0]} table rows")
+    elif slots.shape[0] != n:
+        raise ValueError(f"cu_q describes {n} sequences, slots {slots.shape[0]}")
+    return _index(cu_q, "cu_q", dev), _index(slots, "slots", dev), n
 
 
 def cache_reserve(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, cu_q: torch.Tensor, page: int,
@@ -264,7 +274,7 @@ def cache_reserve(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, 
     c = _cache(None, None, tables, lens, refs, page)
     cu, sl, n = _batch(cu_q, slots, tables)
     status = torch.empty(1, dtype=torch.int32, device=tables.device)
-    _run(tables.device, lib().tt_cache_reserve, c, cu, sl, n, status.data_ptr())
+    _run(tables.get_device(), lib().tt_cache_reserve, c, cu, sl, n, status.data_ptr())
     return status
 
 
@@ -273,21 +283,25 @@ def _token_strides(t: torch.Tensor):
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
-                 lens: torch.Tensor, cu_q: torch.Tensor, slots: Optional[torch.Tensor] = None) -> None:
+                 lens: torch.Tensor, cu_q: torch.Tensor, slots: Optional[torch.Tensor] = None,
+                 status: Optional[torch.Tensor] = None) -> None:
     """Writes the new tokens' k, v [tokens, kv_heads, hs] into one layer's pages; ``lens`` counts them already.
 
     k and v may be strided views that are dense in their features, or dense in their tokens
-    (``qkv_projection``'s vt as ``vt[0, :, :, :n].permute(2, 0, 1)``).
+    (``qkv_projection``'s vt as ``vt[0, :, :, :n].permute(2, 0, 1)``).  With the ``status`` of the
+    ``cache_reserve`` that made the room, nothing is written where that was refused.
     """
     c = _cache(k_pages, v_pages, tables, lens, None)
-    want = (k.shape[0], c.kv_heads, c.head_dim)
-    _need(k_pages.dim() == 4, "append writes one layer's pages")
-    _need(tuple(k.shape) == want and tuple(v.shape) == want, f"k and v must be [tokens, {want[1]}, {want[2]}]")
-    _need(k.dtype == k_pages.dtype and v.dtype == k_pages.dtype, "k and v must have the pages' dtype")
-    _need(k.device == tables.device and v.device == tables.device, f"k and v must be on {tables.device}")
+    dev, want = tables.get_device(), (k.shape[0], c.kv_heads, c.head_dim)
+    if k_pages.dim() != 4:
+        raise ValueError("append writes one layer's pages")
+    if k.shape != want or v.shape != want:
+        raise ValueError(f"k and v must be [tokens, {want[1]}, {want[2]}]")
+    if k.dtype is not k_pages.dtype or v.dtype is not k_pages.dtype or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError("k and v must have the pages' dtype and device")
     cu, sl, n = _batch(cu_q, slots, tables)
-    _run(tables.device, lib().tt_cache_append, c, k.data_ptr(), _token_strides(k), v.data_ptr(), _token_strides(v),
-         want[0], cu, sl, n)
+    _run(tables.get_device(), lib().tt_cache_append, c, k.data_ptr(), _token_strides(k), v.data_ptr(), _token_strides(v),
+         want[0], cu, sl, n, _index(status, "status", dev))
 
 
 def cache_release(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, page: int,
@@ -295,7 +309,8 @@ def cache_release(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, 
     """Frees the slots (all without ``slots``), or with a window the pages that no later query of them can see."""
     c = _cache(None, None, tables, lens, refs, page)
     n = tables.shape[0] if slots is None else slots.shape[0]
-    _run(tables.device, lib().tt_cache_release, c, _index(slots, "slots", tables.device), n, int(window), int(sinks))
+    dev = tables.get_device()
+    _run(dev, lib().tt_cache_release, c, _index(slots, "slots", dev), n, int(window), int(sinks))
 
 
 def cache_fork(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
@@ -306,10 +321,10 @@ def cache_fork(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tenso
     its last page, -2 a bad slot, -3 a child that is not empty or occurs twice.
     """
     c = _cache(k_pages, v_pages, tables, lens, refs)
-    dev = tables.device
+    dev = tables.get_device()
     _need(parents.shape == children.shape, "parents and children must have one length")
     n = parents.shape[0]
-    buf = torch.empty(2 * n + 2, dtype=torch.int32, device=dev)
+    buf = torch.empty(2 * n + 2, dtype=torch.int32, device=tables.device)
     status = buf[:1]
     _run(dev, lib().tt_cache_fork, c, _index(parents, "parents", dev), _index(children, "children", dev), n,
          buf.data_ptr() + 4, status.data_ptr())
@@ -322,7 +337,7 @@ def cache_compact(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Te
     c = _cache(k_pages, v_pages, tables, lens, refs)
     buf = torch.empty(3 * c.n_pages + 3, dtype=torch.int32, device=tables.device)
     live = buf[:1]
-    _run(tables.device, lib().tt_cache_compact, c, buf.data_ptr() + 4, live.data_ptr())
+    _run(tables.get_device(), lib().tt_cache_compact, c, buf.data_ptr() + 4, live.data_ptr())
     return live
 
 
@@ -330,7 +345,7 @@ def cache_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch
                      src: torch.Tensor, dst: torch.Tensor) -> None:
     """Copies pages src[i] -> dst[i] of every layer (no destination twice, none of them a source)."""
     c = _cache(k_pages, v_pages, tables, lens, None)
-    dev = tables.device
+    dev = tables.get_device()
     _need(src.shape == dst.shape, "src and dst must have one length")
     _run(dev, lib().tt_cache_copy_pages, c, _index(src, "src", dev), _index(dst, "dst", dev), src.shape[0])
 
@@ -338,15 +353,12 @@ def cache_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch
 _paged_ws_bytes: Dict[tuple, int] = {}
 
 
-def _paged_workspace(device: torch.device, heads: int, kv_heads: int, head_dim: int, max_q_len: int) -> torch.Tensor:
-    key = (device.index, heads, kv_heads, head_dim, max_q_len)
-    need = _paged_ws_bytes.get(key)
-    if need is None:
-        nbytes = c_size_t()
-        with torch.cuda.device(device):
-            check(lib().tt_paged_attention_workspace_bytes(heads, kv_heads, head_dim, max_q_len, nbytes))
-        need = _paged_ws_bytes[key] = int(nbytes.value)
-    return torch.empty(need, dtype=torch.uint8, device=device)
+def _paged_workspace_bytes(device: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    nbytes = c_size_t()
+    with torch.cuda.device(device):
+        check(lib().tt_paged_attention_workspace_bytes(heads, kv_heads, head_dim, 0, nbytes))
+    _paged_ws_bytes[device, heads, kv_heads, head_dim] = int(nbytes.value)
+    return int(nbytes.value)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
@@ -362,25 +374,31 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``head_dim`` 8 takes pages stored 16 wide; ``max_q_len``, if known, bounds every T.
     """
     c = _cache(k_pages, v_pages, tables, lens, None)
-    dev = tables.device
-    _need(k_pages.dim() == 4, "attention reads one layer's pages")
-    _need(q.dim() == 3 and q.shape[2] == c.head_dim, f"q must be [tokens, heads, {c.head_dim}]")
-    _need(q.dtype == k_pages.dtype and q.device == dev, "q must have the pages' dtype and device")
+    dev = tables.get_device()
     n, heads, hs = q.shape
     st = q.stride()
-    _need(st[2] == 1 or n == 0, "q must be dense in its features")
-    _need(heads % c.kv_heads == 0, f"{heads} query heads are not a multiple of {c.kv_heads} KV heads")
+    if k_pages.dim() != 4:
+        raise ValueError("attention reads one layer's pages")
+    if hs != c.head_dim or (n > 0 and st[2] != 1):
+        raise ValueError(f"q must be [tokens, heads, {c.head_dim}], dense in its features")
+    dtype = q.dtype
+    if dtype is not k_pages.dtype or q.get_device() != dev:
+        raise ValueError("q must have the pages' dtype and device")
+    if heads % c.kv_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {c.kv_heads} KV heads")
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
     hd = hs if head_dim is None else int(head_dim)
-    _need(window >= 0 and sinks >= 0, "window and sinks must not be negative")
     cu, sl, batch = _batch(cu_q, slots, tables)
     if out is None:
-        out = torch.empty(n, heads * hd, dtype=q.dtype, device=dev)
-    else:
-        _need(out.shape == (n, heads * hd) and out.dtype == q.dtype and out.device == dev and out.is_contiguous(),
-              f"out must be a contiguous [{n}, {heads * hd}] tensor of q's dtype on {dev}")
-    bound = n if max_q_len is None else int(max_q_len)
-    ws = _paged_workspace(dev, heads, c.kv_heads, hd, 0)
+        out = torch.empty(n, heads * hd, dtype=dtype, device=q.device)
+    elif (out.shape != (n, heads * hd) or out.dtype is not dtype or out.get_device() != dev or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous [{n}, {heads * hd}] tensor of q's dtype on cuda:{dev}")
+    need = _paged_ws_bytes.get((dev, heads, c.kv_heads, hd))
+    if need is None:
+        need = _paged_workspace_bytes(dev, heads, c.kv_heads, hd)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     _run(dev, lib().tt_paged_attention, c, q.data_ptr(), st[0], st[1], cu, sl, batch, out.data_ptr(), n, heads, hd,
-         q.dtype is torch.bfloat16, hd ** -0.5 if scale is None else float(scale), window, sinks, bound, ws.data_ptr(),
-         ws.numel())
+         dtype is torch.bfloat16, hd ** -0.5 if scale is None else scale, window, sinks,
+         n if max_q_len is None else max_q_len, ws.data_ptr(), need)
     return out
