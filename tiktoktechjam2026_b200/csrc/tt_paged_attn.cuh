@@ -210,14 +210,16 @@ struct PagedWalk {
   __device__ __forceinline__ bool begin(const PagedParams& p, const PagedCut& c, const PagedCut& e, int tpi) {
     end_b = p.batch;
     if (c.b < 0) return false;
-    if (e.b >= 0) {
-      seek(p, e, tpi);
-      end_b = b;
-      end_kvh = kvh;
-      end_qt = qt;
-      end_i = i;
+#pragma unroll 1
+    for (int k = e.b >= 0 ? 0 : 1; k < 2; ++k) {  // the end, then the beginning (one copy of the code)
+      seek(p, k == 0 ? e : c, tpi);
+      if (k == 0) {
+        end_b = b;
+        end_kvh = kvh;
+        end_qt = qt;
+        end_i = i;
+      }
     }
-    seek(p, c, tpi);
     i1 = at_end() ? end_i : it.n;
     return i < i1;
   }
@@ -250,46 +252,54 @@ __device__ __forceinline__ void paged_schedule(const PagedParams& p, int tpi, in
   constexpr int NWARPS = THREADS / 32;
   __shared__ long long warp_sum[NWARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto length = [&](int b) -> long long {
-    if (b >= p.batch) return 0;
-    const PagedSeq s = paged_seq(p, b);
-    const int nq = paged_q_tiles(p, s, tpi);
-    return nq == 0 ? 0 : PagedLine<TK>(p, s, nq, tpi).all() * p.kv_heads;
-  };
-  const long long mine = length(tid);  // kept for the scan below: most batches are one round
-  long long sum = mine;
-  for (int b = tid + THREADS; b < p.batch; b += THREADS) sum += length(b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  if (lane == 0) warp_sum[warp] = sum;
   if (tid < NC) cuts[tid].b = -1;
-  __syncthreads();
-  long long all = 0;
-  for (int w = 0; w < NWARPS; ++w) all += warp_sum[w];
-  const long long each = max(div_pos(all + p.n_workers - 1, p.n_workers), static_cast<long long>(min_tiles) * TK);
-  *per = each;
-  long long carry = 0;
-  for (int b0 = 0; b0 < p.batch && all > 0; b0 += THREADS) {
-    const int b = b0 + tid;
-    const long long u = b0 == 0 ? mine : length(b);
-    long long inc = u;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(~0u, inc, o);
-      if (lane >= o) inc += v;
-    }
-    __syncthreads();  // warp_sum is reread above and in the previous round
-    if (lane == 31) warp_sum[warp] = inc;
-    __syncthreads();
-    long long before = carry;
-    for (int w = 0; w < warp; ++w) before += warp_sum[w];
-    for (int w = 0; w < NWARPS; ++w) carry += warp_sum[w];
-    const long long lo = before + inc - u, hi = before + inc;
+  long long lo = 0, hi = 0, carry = 0, each = 0;  // this thread's sequence lies at lo .. hi on the line
+  int b = 0;
+  auto mark = [&]() {
     for (int w = 0; w < NC; ++w) {
       const long long cut = (first_worker + w) * each;
       if (cut >= lo && cut < hi) cuts[w] = {b, cut - lo};
     }
+  };
+  // One round per THREADS sequences; a second pass, with the length known, only
+  // for batches of more than one round.  (The loops stay rolled: their code
+  // stands in every kernel.)
+#pragma unroll 1
+  for (int pass = 0; pass < (p.batch <= THREADS ? 1 : 2); ++pass) {
+    carry = 0;
+#pragma unroll 1
+    for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
+      b = b0 + tid;
+      long long u = 0;
+      if (b < p.batch) {
+        const PagedSeq s = paged_seq(p, b);
+        const int nq = paged_q_tiles(p, s, tpi);
+        if (nq > 0) u = PagedLine<TK>(p, s, nq, tpi).all() * p.kv_heads;
+      }
+      long long inc = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(~0u, inc, o);
+        if (lane >= o) inc += v;
+      }
+      __syncthreads();  // the round before has read warp_sum
+      if (lane == 31) warp_sum[warp] = inc;
+      __syncthreads();
+      long long before = carry;
+#pragma unroll 1
+      for (int w = 0; w < NWARPS; ++w) {
+        if (w == warp) before = carry;
+        carry += warp_sum[w];
+      }
+      lo = before + inc - u;
+      hi = before + inc;
+      if (pass == 1) mark();
+    }
+    if (pass == 0)
+      each = max(div_pos(carry + p.n_workers - 1, p.n_workers), static_cast<long long>(min_tiles) * TK);
   }
+  if (p.batch <= THREADS) mark();
+  *per = each;
   __syncthreads();
 }
 

@@ -17,7 +17,8 @@
 // maximum m moves only when a tile exceeds it by 2^8 (then O and l are
 // rescaled), and S runs up to NSB - 1 tiles ahead.  At head_dim 128 the tensor
 // core bounds it: key tiles of 128 keep the Q operand's shared-memory reads at
-// the rate of the MMA (64-wide ones read 1.5 times what the pipe can fetch).
+// the rate of the MMA (64-wide ones read 1.5 times what the pipe can fetch),
+// and P.V of a tile's first 64 keys runs while the others' exponentials do.
 // A half skips the tiles that none of its rows sees.
 // The rows of V past a sequence's end in its last page may hold anything
 // (0 * NaN would reach the sum): a spare warp zeroes them in shared memory.
@@ -35,8 +36,8 @@ struct PagedChunkLayout {
   static constexpr int NT = HD == 256 ? 1 : 2;      // halves
   static constexpr int ROWS = 128 * NT;             // rows of a workspace slot
   static constexpr int BN = 64;                     // keys per tile
-  static constexpr int NSB = HD >= 128 ? 2 : 3;      // S buffers per half
-  static constexpr int NST = HD == 256 ? 2 : HD == 128 ? 5 : 8;   // stages of a K and a V tile
+  static constexpr int NSB = HD >= 128 ? 2 : 3;     // S buffers per half
+  static constexpr int NST = HD == 256 ? 2 : HD == 128 ? 5 : 8;  // stages of a K and a V tile
   static constexpr int NQ = HD >= 128 ? 1 : 2;      // Q tile buffers per half
   static constexpr int NOB = HD <= 32 ? 2 : 1;      // O buffers per half
   static constexpr int ATOM = HD >= 64 ? 64 : HD;   // features per swizzle atom
@@ -44,34 +45,37 @@ struct PagedChunkLayout {
   static constexpr int ROW = ATOM * 2;              // bytes of an atom's row
   static constexpr int Q_ATOM = 128 * ROW, KV_ATOM = BN * ROW;
   static constexpr int Q_BYTES = NATOM * Q_ATOM, KV_BYTES = NATOM * KV_ATOM;
+  // Segments published ahead: the scores may be NSB segments of one tile
+  // before the one whose P.V is under way, and the producer ahead of them.
+  static constexpr int NSEG = 6;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = NT * NQ * Q_BYTES;
   static constexpr int OFF_V = OFF_K + NST * KV_BYTES;
   static constexpr int OFF_BAR = OFF_V + NST * KV_BYTES;
-  // Barriers: stage full / empty / stale rows zeroed, then per half Q
-  // full / empty, S full, P full, O full / free, done.
-  static constexpr int B_F = 0, B_E = NST, B_X = 2 * NST, B_HALF = 3 * NST;
-  static constexpr int H_QF = 0, H_QE = 2, H_SF = 4, H_PF = H_SF + NSB, H_OF = H_PF + NSB, H_OR = H_OF + 2,
-                       H_DONE = H_OR + 2, N_HALF = H_DONE + 1;
+  // Barriers: stage full / empty / stale rows zeroed, segment full / empty, then
+  // per half Q full / empty, S full, P full, P.V done, O full / free, drained.
+  static constexpr int B_F = 0, B_E = NST, B_X = 2 * NST, B_GF = 3 * NST, B_GE = B_GF + NSEG, B_HALF = B_GE + NSEG;
+  static constexpr int H_QF = 0, H_QE = 2, H_SF = 4, H_PF = H_SF + NSB, H_PE = H_PF + NSB, H_OF = H_PE + NSB,
+                       H_OR = H_OF + 2, H_DONE = H_OR + 2, N_HALF = H_DONE + 2;
   static constexpr int OFF_MISC = OFF_BAR + (B_HALF + NT * N_HALF) * 8;
   static constexpr int SMEM = OFF_MISC + 16 + 1024;
   static constexpr int TMEM_COLS = 512, TMEM_O = NSB * BN, TMEM_HALF = 512 / NT;
-  static constexpr int W_PROD = 4 * NT, W_FIX = W_PROD + 1, W_MMA = W_PROD + 2;  // MMA warps: W_MMA + half
-  static constexpr int NWARPS = NT == 2 ? 12 : 8;
+  // Warps: softmax (half w / 4, lane quadrant w % 4), producer, score and P.V
+  // issuers of each half, idle ones up to whole warpgroups (setmaxnreg).
+  static constexpr int W_PROD = 4 * NT, W_S = W_PROD + 1, W_PV = W_S + NT;
+  static constexpr int NWARPS = NT == 2 ? 16 : 8;
   static constexpr int THREADS = 32 * NWARPS;
   // Register split (setmaxnreg): the launch provides THREADS x REGS_LAUNCH and
   // the launcher refuses to start a kernel built with another count (a split
-  // above the launch total would make setmaxnreg.inc wait forever).  The MMA
-  // warps carry two walks of the piece, the softmax warps a row of BN scores.
+  // above the launch total would make setmaxnreg.inc wait forever).
   static constexpr bool SPLIT = NT == 2;
-  static constexpr int REGS_LAUNCH = 168;
-  static constexpr int REGS_SOFTMAX = 184, REGS_OTHER = 136;
+  static constexpr int REGS_LAUNCH = 128;
+  static constexpr int REGS_SOFTMAX = 184, REGS_OTHER = 72;
   static_assert(!SPLIT || 128 * NT * REGS_SOFTMAX + 32 * (NWARPS - 4 * NT) * REGS_OTHER <= THREADS * REGS_LAUNCH,
                 "register split");
-  // A stage is waited for while the NSB before it but one are held.
-  static_assert(NST >= NSB, "ring depth");
+  static_assert(NSEG >= NSB + 2, "ring depth");
   static_assert(TMEM_O + NOB * HD <= TMEM_HALF, "TMEM budget");
-  static_assert(SMEM <= 232448, "shared memory budget");
+  static_assert(SMEM <= 232448 - 1280, "shared memory budget (the rest is static)");
   static_assert(Q_BYTES % 1024 == 0 && KV_BYTES % 1024 == 0 && OFF_BAR % 1024 == 0, "alignment");
 };
 
@@ -127,61 +131,95 @@ __device__ __forceinline__ uint32_t bits_below(int x) {  // the lowest x bits (n
   return x >= 32 ? ~0u : (x <= 0 ? 0u : (1u << x) - 1u);
 }
 
-// The tiles of an item that some row of one half sees, as ranges of the item's
-// tile index: [0, a) and [c, e).
-struct ChunkRange {
-  int a, c, e;
-  __device__ __forceinline__ bool has(int i) const { return i < a || (i >= c && i < e); }
-  // Last such tile of [i0, i1), or -1.
-  __device__ __forceinline__ int last(int i0, int i1) const {
-    const int y = min(e, i1) - 1;
-    if (y >= max(c, i0)) return y;
-    const int x = min(a, i1) - 1;
-    return x >= i0 ? x : -1;
-  }
-};
-
-// One half of a segment (a segment is the part of one item that lies in the piece).
+// A segment is the part of one item that lies in the worker's piece.  The
+// producer warp walks the piece and publishes each segment, one ahead of the
+// tiles it fetches, for the other warps: the walk's code exists once (the
+// warps' hot loops have to share the instruction cache).
 struct ChunkHalf {
-  int rows;        // query rows
-  int p0, p1;      // positions of the first and last row
-  ChunkRange range;
-  int last;        // the last tile of the segment that it sees, -1: none
+  int rows;      // query rows
+  int p0, p1;    // positions of the first and last row
+  int a, c, e;   // the item's tiles that some row sees: [0, a) and [c, e)
+  int last;      // the last of them in the segment, -1: none
+};
+struct ChunkSegment {
+  int i0, i1;           // tiles of the item (i1 < 0: the piece has ended)
+  int n_sink, w_shift;  // tile i is key tile i, or i + w_shift from n_sink on
+  int whole;            // the segment is a whole item
+  int kvh, tok, slot, keys;  // KV head, row of q of the first token, table row, length
+  int fix_at, fix_r0, fix_r1;  // tile (-1: none) whose V rows fix_r0 .. fix_r1 - 1 lie past the sequence's end
+  ChunkHalf half[2];
+  __device__ __forceinline__ int key(int i, int bn) const { return (i < n_sink ? i : i + w_shift) * bn; }
 };
 
-// Walks a worker's piece; a segment is the part of one item that lies in it.
 template <int HD>
-struct ChunkWalk : PagedWalk<PagedChunkLayout<HD>::BN> {
-  static constexpr int BN = PagedChunkLayout<HD>::BN;
-  __device__ __forceinline__ ChunkHalf half(const PagedParams& p, int h, int half_tokens) const {
-    ChunkHalf x;
+__device__ __forceinline__ void chunk_segment(const PagedParams& p, const PagedWalk<PagedChunkLayout<HD>::BN>& w,
+                                           int half_tokens, ChunkSegment* out) {
+  using L = PagedChunkLayout<HD>;
+  constexpr int BN = L::BN;
+  ChunkSegment g;
+  g.i0 = w.i;
+  g.i1 = w.i1;
+  g.n_sink = w.it.n_sink;
+  g.w_shift = w.it.w_tile - w.it.n_sink;
+  g.whole = w.i == 0 && w.i1 == w.it.n;
+  g.kvh = w.kvh;
+  g.tok = w.s.q0 + w.it.r0 / p.group;
+  g.slot = w.s.slot;
+  g.keys = w.s.L;
+  // Only the item's last tile can hold the sequence's end.
+  const int page = 1 << p.page_shift, r0 = w.s.L - w.it.tile(w.it.n - 1) * BN;
+  g.fix_r0 = r0;
+  g.fix_r1 = min((r0 + page - 1) & ~(page - 1), BN);  // the end of its page, or of the tile
+  g.fix_at = r0 > 0 && r0 < BN && (r0 & (page - 1)) != 0 ? w.it.n - 1 : -1;
+  for (int h = 0; h < L::NT; ++h) {
+    ChunkHalf x = {};
     const int hr = half_tokens * p.group;
-    x.rows = min(max(this->it.rows - h * hr, 0), hr);
-    x.range = {0, 0, 0};
+    x.rows = min(max(w.it.rows - h * hr, 0), hr);
     x.last = -1;
-    x.p0 = this->it.p0 + h * half_tokens;
-    x.p1 = x.p0 + (x.rows - 1) / p.group;
-    if (x.rows == 0) return x;
-    const int end = x.p1 < 0 ? 0 : x.p1 / BN + 1;  // one past the last tile a row sees
-    if (p.window == 0) {
-      x.range.e = end;
-    } else {
-      const int from = max(x.p0 - p.window + 1, 0) / BN;  // first tile in the window
-      const int sink = (min(p.sinks, BN * end) + BN - 1) / BN;
-      if (this->it.n_sink == this->it.n) {  // no gap: the index is the tile
-        x.range.a = min(sink, end);
-        x.range.c = max(from, x.range.a);
-        x.range.e = end;
+    if (x.rows > 0) {
+      x.p0 = w.it.p0 + h * half_tokens;
+      x.p1 = x.p0 + (x.rows - 1) / p.group;
+      const int end = x.p1 < 0 ? 0 : x.p1 / BN + 1;  // one past the last tile a row sees
+      if (p.window == 0) {
+        x.e = end;
       } else {
-        x.range.a = min(this->it.n_sink, end);
-        x.range.c = max(from - this->it.w_tile, 0) + this->it.n_sink;
-        x.range.e = end - this->it.w_tile + this->it.n_sink;
+        const int from = max(x.p0 - p.window + 1, 0) / BN;  // first tile in the window
+        const int sink = (min(p.sinks, BN * end) + BN - 1) / BN;
+        if (w.it.n_sink == w.it.n) {  // no gap: the index is the tile
+          x.a = min(sink, end);
+          x.c = max(from, x.a);
+          x.e = end;
+        } else {
+          x.a = min(w.it.n_sink, end);
+          x.c = max(from - w.it.w_tile, 0) + w.it.n_sink;
+          x.e = end - w.it.w_tile + w.it.n_sink;
+        }
       }
+      const int y = min(x.e, w.i1) - 1, z = min(x.a, w.i1) - 1;
+      x.last = y >= max(x.c, w.i) ? y : (z >= w.i ? z : -1);
     }
-    x.last = x.range.last(this->i, this->i1);
-    return x;
+    g.half[h] = x;
   }
-};
+  *out = g;
+}
+
+// wait_phase in few instructions (there are some twenty waits in the kernel).
+__device__ __forceinline__ bool chunk_wait(uint64_t* bar, uint32_t parity, const Watchdog& wd, uint32_t site) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    const bool late = globaltimer_ns() - t0 > wd.timeout_ns;
+    if (late) atomicCAS(wd.err, 0u, kDevErrTimeout | (site & 0xffffu));
+    if (late || *wd.abort || grid_failed(wd)) {
+      *wd.abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ bool chunk_wait_warp(uint64_t* bar, uint32_t parity, const Watchdog& wd, uint32_t site) {
+  return __all_sync(0xffffffffu, chunk_wait(bar, parity, wd, site));
+}
 
 // Exponentials per 8 pairs on the FMA pipe.
 template <int HD>
@@ -197,18 +235,18 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   constexpr int BN = L::BN, NT = L::NT, NSB = L::NSB, NST = L::NST, NQ = L::NQ, NOB = L::NOB;
   extern __shared__ uint8_t smem_raw[];
   __shared__ PagedCut cuts[2];
-  __shared__ ChunkWalk<HD> saved[6 * NT];  // walks at rest: the softmax warps', then two of each MMA warp
+  __shared__ PagedWalk<BN> walk;  // the producer's
+  __shared__ ChunkSegment segments[L::NSEG];
+  __shared__ bool any;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half_rows = half_tokens * p.group, tpi = NT * half_tokens;
   long long per;
   paged_schedule<BN, 2, L::THREADS>(p, tpi, min_tiles, blockIdx.x, cuts, &per);
   paged_zero_outside(p, L::THREADS);
   pdl_trigger();
-  __shared__ bool any;
-  if (threadIdx.x == 0) any = saved[0].begin(p, cuts[0], cuts[1], tpi);
+  if (threadIdx.x == 0) any = walk.begin(p, cuts[0], cuts[1], tpi);
   __syncthreads();
   if (!any) return;
-  ChunkWalk<HD> walk = saved[0];
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -218,8 +256,12 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < NST; ++i) {
       mbar_init(&bars[L::B_F + i], 1);
-      mbar_init(&bars[L::B_E + i], NT + 1);  // the MMA warps and the warp that zeroes stale rows
+      mbar_init(&bars[L::B_E + i], NT);
       mbar_init(&bars[L::B_X + i], 1);
+    }
+    for (int i = 0; i < L::NSEG; ++i) {
+      mbar_init(&bars[L::B_GF + i], 1);
+      mbar_init(&bars[L::B_GE + i], 6 * NT);  // softmax warps and issuers
     }
     for (int h = 0; h < NT; ++h) {
       uint64_t* b = bars + L::B_HALF + h * L::N_HALF;
@@ -232,13 +274,15 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
       for (int i = 0; i < NSB; ++i) {
         mbar_init(&b[L::H_SF + i], 1);
         mbar_init(&b[L::H_PF + i], 4);
+        mbar_init(&b[L::H_PE + i], 1);
       }
       mbar_init(&b[L::H_DONE], 1);
+      mbar_init(&b[L::H_DONE + 1], 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == L::W_MMA) {
+  if (warp == L::W_S) {
     tmem_alloc(tmem_slot, L::TMEM_COLS);
     tmem_relinquish();
   }
@@ -248,6 +292,18 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   const uint32_t tmem_base = *tmem_slot;
   const Watchdog wd{p.err, abort_flag, p.timeout_ns};
   const int page_rows = 1 << p.page_shift;
+
+  // A consumer's place in the ring of segments.
+  struct Place {
+    int at = 0;
+    uint32_t ph = 0;
+    __device__ __forceinline__ void step() {
+      if (++at == L::NSEG) {
+        at = 0;
+        ph ^= 1;
+      }
+    }
+  };
 
   if (warp == L::W_PROD) {
     // -------------------------------------------------------------- producer
@@ -260,44 +316,62 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     const int box = min(page_rows, BN), n_box = BN / box;  // boxes of a tile: lane i fetches the i-th
     int u = 0, st = 0, nq[NT] = {};
     uint32_t ph = 0;
+    Place put, get;
+    bool more = true;  // the walk stands on a segment that is not published yet
     bool ok = true;
-    do {
+    for (bool started = false;; started = true) {
+      // Publishes the walk's segment (or the end) and moves the walk on.
+      if (!(ok = chunk_wait_warp(&bars[L::B_GE + put.at], put.ph ^ 1, wd, 0x530))) break;
+      if (lane == 0) {
+        if (more) {
+          chunk_segment<HD>(p, walk, half_tokens, &segments[put.at]);
+          more = walk.next(p, tpi);
+        } else {
+          segments[put.at].i1 = -1;
+        }
+        mbar_arrive(&bars[L::B_GF + put.at]);
+      }
+      __syncwarp();
+      more = __shfl_sync(~0u, more, 0);
+      put.step();
+      if (!started) continue;  // the segment after the one in hand is always published
+      const ChunkSegment& g = segments[get.at];
+      get.step();
+      if (g.i1 < 0) break;
 #pragma unroll
       for (int h = 0; h < NT; ++h) {
-        if (walk.half(p, h, half_tokens).last < 0) continue;
+        if (g.half[h].last < 0) continue;
         uint64_t* b = bars + L::B_HALF + h * L::N_HALF;
         const int qb = nq[h] % NQ;
-        if (lane == 0) ok = wait_phase(&b[L::H_QE + qb], ((nq[h] / NQ) & 1) ^ 1, wd, 0x531);
-        if (!(ok = __shfl_sync(~0u, ok, 0))) break;
+        if (!(ok = chunk_wait_warp(&b[L::H_QE + qb], ((nq[h] / NQ) & 1) ^ 1, wd, 0x531))) break;
         if (lane == 0) {
-          const int tok = walk.s.q0 + walk.it.r0 / p.group + h * half_tokens;
           mbar_arrive_expect_tx(&b[L::H_QF + qb], L::NATOM * half_rows * L::ROW);
 #pragma unroll
           for (int a = 0; a < L::NATOM; ++a)
             tma_load_3d(smem + L::OFF_Q + (h * NQ + qb) * L::Q_BYTES + a * L::Q_ATOM, &tmQ, &b[L::H_QF + qb],
-                        a * L::ATOM, walk.kvh * p.group, tok);
+                        a * L::ATOM, g.kvh * p.group, g.tok + h * half_tokens);
         }
         ++nq[h];
       }
       if (!ok) break;
-      const int* row = p.tables + walk.s.slot * p.table_stride;
-      const int n_keys = walk.s.L;
-      // The page of this lane's box of tile i (n_pages, past the end, where there is none).
-      auto page_of = [&](int i) -> int {
-        const int key = walk.it.tile(i) * BN + lane * box;
+      const int* row = p.tables + g.slot * p.table_stride;
+      const int n_keys = g.keys, row0 = g.kvh * page_rows, i1 = g.i1, n_sink = g.n_sink, w_shift = g.w_shift;
+      // First key of this lane's box of tile i, and its page (n_pages, past the pool's end, where there is none).
+      auto key_of = [&](int i) -> int { return (i < n_sink ? i : i + w_shift) * BN + lane * box; };
+      auto page_of = [&](int key) -> int {
         int pg = -1;
         if (lane < n_box && key < n_keys) pg = row[key >> p.page_shift];
         return pg < 0 || pg >= p.n_pages ? p.n_pages : pg;
       };
-      int page = page_of(walk.i);
-      for (int i = walk.i; i < walk.i1; ++i, ++u) {
-        const int next = i + 1 < walk.i1 ? page_of(i + 1) : 0;  // a tile ahead: its latency is off the path
-        const int at = walk.kvh * page_rows + ((walk.it.tile(i) * BN + lane * box) & (page_rows - 1));
-        if (lane == 0) {
-          ok = wait_phase(&bars[L::B_E + st], ph ^ 1, wd, 0x532);
-          if (ok) mbar_arrive_expect_tx(&bars[L::B_F + st], 2 * L::KV_BYTES);
-        }
-        if (!(ok = __shfl_sync(~0u, ok, 0))) break;
+      int key = key_of(g.i0), page = page_of(key);
+#pragma unroll 1
+      for (int i = g.i0; i < i1; ++i, ++u) {
+        const int next_key = key_of(i + 1);
+        const int next = i + 1 < i1 ? page_of(next_key) : 0;  // a tile ahead: its latency is off the path
+        const int at = row0 + (key & (page_rows - 1));
+        if (!(ok = chunk_wait_warp(&bars[L::B_E + st], ph ^ 1, wd, 0x532))) break;
+        if (lane == 0) mbar_arrive_expect_tx(&bars[L::B_F + st], 2 * L::KV_BYTES);
+        __syncwarp();
         if (lane < n_box) {
           uint8_t* dst = smem + L::OFF_K + st * L::KV_BYTES + lane * box * L::ROW;
 #pragma unroll
@@ -311,10 +385,11 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
           st = 0;
           ph ^= 1;
         }
-        if (!ok) break;
+        key = next_key;
         page = next;
       }
-    } while (ok && walk.next(p, tpi));
+      if (!ok) break;
+    }
     // Let every copy this warp started land before the CTA may exit.
     if (lane == 0) {
       for (int h = 0; h < NT; ++h)
@@ -322,174 +397,136 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
           wait_drain(&bars[L::B_HALF + h * L::N_HALF + L::H_QF + i % NQ], (i / NQ) & 1, kDrainLimitNs);
       for (int i = max(u - NST, 0); i < u; ++i) wait_drain(&bars[L::B_F + i % NST], (i / NST) & 1, kDrainLimitNs);
     }
-  } else if (warp == L::W_FIX) {
-    // -------------------------------------------------------------- zeroes the stale rows of V
+  } else if (warp >= L::W_S && warp < L::W_S + 2 * NT) {
+    // -------------------------------------------------------------- issuers of a half
+    // Scores and P.V are issued by warps of their own: an issuer's loop is a
+    // chain of waits and short bursts, and one warp doing both took longer per
+    // tile than the softmax.  A warp walks its loop as a whole on values that
+    // shuffles make warp-uniform, and one elected lane issues: in a region of a
+    // single lane every operand would go through vector registers.
     if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_OTHER));
-    int st = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    do {
-      // Only the item's last tile can hold the end of the sequence.
-      const int r0 = walk.s.L - walk.it.tile(walk.it.n - 1) * BN;
-      const int r1 = min((r0 + page_rows - 1) & ~(page_rows - 1), BN);  // the end of its page, or of the tile
-      const int fix_at = r0 > 0 && r0 < BN && (r0 & (page_rows - 1)) != 0 ? walk.it.n - 1 : -1;
-      for (int i = walk.i; i < walk.i1; ++i) {
-        if (!(ok = warp_wait_phase(&bars[L::B_F + st], ph, wd, 0x534))) break;
-        if (i == fix_at) {
-          const uint32_t base = smem_u32(smem + L::OFF_V + st * L::KV_BYTES);
-          for (int a = 0; a < L::NATOM; ++a)
-            for (int x = r0 * L::ROW + lane * 16; x < r1 * L::ROW; x += 512)
-              st_shared_v4(base + a * L::KV_ATOM + x, 0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[L::B_X + st]);
-        }
-        if (lane == 0) mbar_arrive(&bars[L::B_E + st]);
-        if (++st == NST) {
-          st = 0;
-          ph ^= 1;
-        }
-      }
-    } while (ok && walk.next(p, tpi));
-  } else if (warp >= L::W_MMA && warp < L::W_MMA + NT) {
-    // -------------------------------------------------------------- MMA issuer of a half
-    // The warp's own instructions are on the critical path.  It walks the loop
-    // as a whole on values that shuffles and votes make warp-uniform, and one
-    // elected lane issues: in a region of a single lane every operand would go
-    // through vector registers.
-    if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_OTHER));
-    const int h = __shfl_sync(~0u, warp - L::W_MMA, 0);
+    const bool scores = warp < L::W_PV;
+    const int h = __shfl_sync(~0u, warp - (scores ? L::W_S : L::W_PV), 0);
     uint64_t* b = bars + L::B_HALF + h * L::N_HALF;
     const uint32_t sbase = smem_u32(smem);
     constexpr uint32_t kSw = swizzle_kind_for_bytes(L::ROW), kSbo = 8 * L::ROW;
-    constexpr uint32_t idesc_s = umma_idesc_16(128, BN, PT::kBf16, false);
-    constexpr uint32_t idesc_o = umma_idesc_16(128, HD, PT::kBf16, true);
-    const uint64_t dq0 = umma_sdesc(sbase + L::OFF_Q + h * NQ * L::Q_BYTES, kSbo, kSw);
-    const uint64_t dk0 = umma_sdesc(sbase + L::OFF_K, kSbo, kSw);
-    const uint64_t dv0 = umma_sdesc_mn(sbase + L::OFF_V, L::KV_ATOM, kSbo, kSw);
     const uint32_t tS = __shfl_sync(~0u, tmem_base, 0) + h * L::TMEM_HALF;
-    // Two walks of the piece, in shared memory: [0] for the scores, which run
-    // NSB units ahead (counted in units and not in the half's tiles: the producer
-    // can then always fill what is waited for), [1] for P.V.
-    ChunkWalk<HD>* walks = saved + 4 * NT + 2 * h;
-    struct Segment {  // warp-uniform
-      int i, i1, a, c, e, last, fix_at;
-      __device__ __forceinline__ bool has() const { return i < a || (i >= c && i < e); }
-    };
-    auto read = [&](const ChunkWalk<HD>& w) -> Segment {
-      const ChunkHalf x = w.half(p, h, half_tokens);
-      const int r0 = w.s.L - w.it.tile(w.it.n - 1) * BN;
-      const int fix = r0 > 0 && r0 < BN && (r0 & (page_rows - 1)) != 0 ? w.it.n - 1 : -1;
-      return {__shfl_sync(~0u, w.i, 0),       __shfl_sync(~0u, w.i1, 0),      __shfl_sync(~0u, x.range.a, 0),
-              __shfl_sync(~0u, x.range.c, 0), __shfl_sync(~0u, x.range.e, 0), __shfl_sync(~0u, x.last, 0),
-              __shfl_sync(~0u, fix, 0)};
-    };
-    if (lane == 0) {
-      walks[0] = walk;
-      walks[1] = walk;
-    }
-    __syncwarp();
-    Segment ss = read(walks[0]);
-    int k_st = 0, s_buf = 0, q_buf = 0;
-    uint32_t k_ph = 0, q_ph = 0;
-    bool more_s = true, q_new = true;
-    // Waits for the next unit's stage and issues its scores, if this half sees it.
-    auto step_s = [&]() -> bool {
-      if (ss.i == ss.i1) {
-        if (!more_s) return true;
-        more_s = __shfl_sync(~0u, lane == 0 ? walks[0].next(p, tpi) : false, 0);
-        __syncwarp();
-        if (!more_s) return true;
-        ss = read(walks[0]);
-        q_new = true;
-      }
-      if (!warp_wait_phase(&bars[L::B_F + k_st], k_ph, wd, 0x536)) return false;
-      if (ss.has()) {
-        if (q_new) {
-          if (!warp_wait_phase(&b[L::H_QF + q_buf], q_ph, wd, 0x535)) return false;
-          q_new = false;
-        }
-        tc_fence_after();
-        const uint64_t dq = dq0 + (q_buf * L::Q_BYTES >> 4), dk = dk0 + (k_st * L::KV_BYTES >> 4);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const int at = 16 * kk / L::ATOM, off = 16 * kk % L::ATOM * 2;
-            umma_f16(tS + s_buf * BN, dq + ((at * L::Q_ATOM + off) >> 4), dk + ((at * L::KV_ATOM + off) >> 4), idesc_s,
-                     kk > 0 ? 1u : 0u);
-          }
-          umma_commit(&b[L::H_SF + s_buf]);
-          if (ss.i == ss.last) umma_commit(&b[L::H_QE + q_buf]);
-        }
-        __syncwarp();
-        if (++s_buf == NSB) s_buf = 0;
-        if (ss.i == ss.last && ++q_buf == NQ) {
-          q_buf = 0;
-          q_ph ^= 1;
-        }
-      }
-      if (++k_st == NST) {
-        k_st = 0;
-        k_ph ^= 1;
-      }
-      ++ss.i;
-      return true;
-    };
+    int st = 0, buf = 0, side = 0;  // stage; S buffer; Q buffer (scores) or O buffer (P.V)
+    uint32_t ph = 0, buf_ph = 0, side_ph = 0;
+    uint32_t fixed = 0;  // parity of the next zeroing of each stage
     bool ok = true;
-    for (int k = 0; ok && k < NSB; ++k) ok = step_s();
-    int v_st = 0, p_buf = 0, o_buf = 0;
-    uint32_t p_ph = 0, o_ph = 0, fixed = 0;  // fixed: parity of the next zeroing of each stage
-    bool more = ok;
-    while (more) {
-      Segment so = read(walks[1]);
-      bool first = true;
-      for (; so.i < so.i1; ++so.i) {
-        const bool on = so.has();
-        if (on) {
-          if (first) ok = warp_wait_phase(&b[L::H_OR + o_buf], o_ph ^ 1, wd, 0x539);
-          ok = ok && warp_wait_phase(&b[L::H_PF + p_buf], p_ph, wd, 0x538);
-        }
-        if (so.i == so.fix_at) {
-          ok = ok && warp_wait_phase(&bars[L::B_X + v_st], (fixed >> v_st) & 1, wd, 0x53b);
-          fixed ^= 1u << v_st;
-        }
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t dv = dv0 + (v_st * L::KV_BYTES >> 4);
-        const uint32_t tO = tS + L::TMEM_O + o_buf * HD, tP = tS + p_buf * BN;
-        if (elect_one()) {
-          if (on) {
-#pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)
-              umma_f16_ts(tO, tP + kk * 8, dv + (kk * 16 * L::ROW >> 4), idesc_o, kk == 0 && first ? 0u : 1u);
-            umma_commit(&bars[L::B_E + v_st]);
-            if (so.i == so.last) umma_commit(&b[L::H_OF + o_buf]);
-          } else {
-            mbar_arrive(&bars[L::B_E + v_st]);  // its stage was full before its scores were passed over
-          }
-        }
-        __syncwarp();
-        if (on) {
-          first = false;
-          if (++p_buf == NSB) {
-            p_buf = 0;
-            p_ph ^= 1;
-          }
-          if (so.i == so.last && ++o_buf == NOB) {
-            o_buf = 0;
-            o_ph ^= 1;
-          }
-        }
-        if (++v_st == NST) v_st = 0;
-        if (!(ok = step_s())) break;
-      }
-      more = ok && __shfl_sync(~0u, lane == 0 ? walks[1].next(p, tpi) : false, 0);
+    Place get;
+    while (ok) {
+      if (!(ok = chunk_wait_warp(&bars[L::B_GF + get.at], get.ph, wd, 0x53e))) break;
+      const ChunkSegment& g = segments[get.at];
+      const ChunkHalf& x = g.half[h];
+      int i = __shfl_sync(~0u, g.i0, 0);
+      const int i1 = __shfl_sync(~0u, g.i1, 0), a = __shfl_sync(~0u, x.a, 0), c = __shfl_sync(~0u, x.c, 0),
+                e = __shfl_sync(~0u, x.e, 0), last = __shfl_sync(~0u, x.last, 0), fix_at = __shfl_sync(~0u, g.fix_at, 0);
+      const int r0 = g.fix_r0, r1 = g.fix_r1;
       __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[L::B_GE + get.at]);
+      get.step();
+      if (i1 < 0) break;
+      bool first = true;
+      if (scores) {
+        constexpr uint32_t idesc = umma_idesc_16(128, BN, PT::kBf16, false);
+        const uint64_t dq0 = umma_sdesc(sbase + L::OFF_Q + h * NQ * L::Q_BYTES, kSbo, kSw);
+        const uint64_t dk0 = umma_sdesc(sbase + L::OFF_K, kSbo, kSw);
+#pragma unroll 1
+        for (; i < i1; ++i) {
+          const bool on = i < a || (i >= c && i < e);
+          if (on && first) ok = chunk_wait_warp(&b[L::H_QF + side], side_ph, wd, 0x535);
+          if (on) ok = ok && chunk_wait_warp(&b[L::H_PE + buf], buf_ph ^ 1, wd, 0x537);
+          if (!(ok = ok && chunk_wait_warp(&bars[L::B_F + st], ph, wd, 0x536))) break;
+          if (h == 0 && i == fix_at) {  // V rows past the sequence's end hold anything: zero them
+            const uint32_t base = smem_u32(smem + L::OFF_V + st * L::KV_BYTES);
+            for (int at = 0; at < L::NATOM; ++at)
+              for (int y = r0 * L::ROW + lane * 16; y < r1 * L::ROW; y += 512)
+                st_shared_v4(base + at * L::KV_ATOM + y, 0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[L::B_X + st]);
+          }
+          if (on) {
+            first = false;
+            tc_fence_after();
+            const uint64_t dq = dq0 + (side * L::Q_BYTES >> 4), dk = dk0 + (st * L::KV_BYTES >> 4);
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < HD / 16; ++kk) {
+                const int at = 16 * kk / L::ATOM, off = 16 * kk % L::ATOM * 2;
+                umma_f16(tS + buf * BN, dq + ((at * L::Q_ATOM + off) >> 4), dk + ((at * L::KV_ATOM + off) >> 4), idesc,
+                         kk > 0 ? 1u : 0u);
+              }
+              umma_commit(&b[L::H_SF + buf]);
+              if (i == last) umma_commit(&b[L::H_QE + side]);
+            }
+            __syncwarp();
+            if (++buf == NSB) {
+              buf = 0;
+              buf_ph ^= 1;
+            }
+            if (i == last && ++side == NQ) {
+              side = 0;
+              side_ph ^= 1;
+            }
+          }
+          if (++st == NST) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+      } else {
+        constexpr uint32_t idesc = umma_idesc_16(128, HD, PT::kBf16, true);
+        const uint64_t dv0 = umma_sdesc_mn(sbase + L::OFF_V, L::KV_ATOM, kSbo, kSw);
+#pragma unroll 1
+        for (; i < i1; ++i) {
+          const bool on = i < a || (i >= c && i < e);
+          if (i == fix_at) {
+            if (!(ok = chunk_wait_warp(&bars[L::B_X + st], (fixed >> st) & 1, wd, 0x53b))) break;
+            fixed ^= 1u << st;
+          }
+          if (on) {
+            if (first) ok = chunk_wait_warp(&b[L::H_OR + side], side_ph ^ 1, wd, 0x539);
+            if (!(ok = ok && chunk_wait_warp(&b[L::H_PF + buf], buf_ph, wd, 0x538))) break;
+            tc_fence_after();
+            const uint64_t dv = dv0 + (st * L::KV_BYTES >> 4);
+            const uint32_t tO = tS + L::TMEM_O + side * HD, tP = tS + buf * BN;
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < BN / 16; ++kk)
+                umma_f16_ts(tO, tP + kk * 8, dv + (kk * 16 * L::ROW >> 4), idesc, kk == 0 && first ? 0u : 1u);
+              umma_commit(&b[L::H_PE + buf]);
+              umma_commit(&bars[L::B_E + st]);
+              if (i == last) umma_commit(&b[L::H_OF + side]);
+            }
+            __syncwarp();
+            first = false;
+            if (++buf == NSB) {
+              buf = 0;
+              buf_ph ^= 1;
+            }
+            if (i == last && ++side == NOB) {
+              side = 0;
+              side_ph ^= 1;
+            }
+          } else {  // not seen by this half: hand the stage back once it is there
+            if (!(ok = chunk_wait_warp(&bars[L::B_F + st], ph, wd, 0x53a))) break;
+            if (lane == 0) mbar_arrive(&bars[L::B_E + st]);
+          }
+          if (++st == NST) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+      }
     }
     // All MMAs the elected lane issued must finish before TMEM is released.
-    if (elect_one()) umma_commit(&b[L::H_DONE]);
+    uint64_t* done = &b[L::H_DONE + (scores ? 0 : 1)];
+    if (elect_one()) umma_commit(done);
     __syncwarp();
-    if (lane == 0) wait_drain(&b[L::H_DONE], 0, kDrainLimitNs);
+    if (lane == 0) wait_drain(done, 0, kDrainLimitNs);
     __syncwarp();
   } else if (warp >= 4 * NT) {
     if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_OTHER));
@@ -515,7 +552,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     int pend_row = 0;
     auto finish = [&]() -> bool {
       pend = false;
-      if (!warp_wait_phase(&b[L::H_OF + pend_o], pend_ph, wd, 0x541)) return false;
+      if (!chunk_wait_warp(&b[L::H_OF + pend_o], pend_ph, wd, 0x541)) return false;
       tc_fence_after();
       const uint32_t tO = tS + L::TMEM_O + pend_o * HD;
       const float inv = pend_l > 1e-30f ? 1.f / pend_l : 0.f;  // (a row that sees a key has l >= 1)
@@ -557,40 +594,36 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
       return true;
     };
 
-    // The walk rests in shared memory while a segment is worked on: its
-    // registers would push the scores out.
-    if (lane == 0) saved[warp] = walk;
-    bool more = true;
-    int units = 0;  // of the segments so far
-    for (; ok && more; more = __shfl_sync(~0u, lane == 0 ? saved[warp].next(p, tpi) : false, 0)) {
-      ChunkRange range;
-      int i, last, p0, p1, pos, n_sink, w_shift, unit;  // unit: ring position of tile i
+    for (Place get; ok; get.step()) {
+      if (!(ok = chunk_wait_warp(&bars[L::B_GF + get.at], get.ph, wd, 0x540))) break;
+      int i, last, p0, p1, pos, n_sink, w_shift, a, c;
       bool on;
       const int item_row = h * half_rows + row;
       T* out = nullptr;
       float* part = nullptr;  // set when the item is cut
-      __syncwarp();           // lane 0's walk is visible
       {
-        const ChunkWalk<HD>& w = saved[warp];
-        const ChunkHalf x = w.half(p, h, half_tokens);
-        range = x.range;
-        i = w.i < range.a ? w.i : max(range.c, w.i);
+        const ChunkSegment& g = segments[get.at];
+        if (g.i1 < 0) break;
+        const ChunkHalf& x = g.half[h];
+        a = x.a;
+        c = x.c;
+        i = g.i0 < a ? g.i0 : max(c, g.i0);
         last = x.last;
-        unit = units + i - w.i;
-        units += w.i1 - w.i;
         p0 = x.p0;
         p1 = x.p1;
-        pos = x.p0 + row / p.group;
+        const int t = row / p.group;
+        pos = p0 + t;
         on = row < x.rows;
-        n_sink = w.it.n_sink;
-        w_shift = w.it.w_tile - n_sink;
-        const int r = w.it.r0 + item_row;
-        const long long tok = w.s.q0 + r / p.group;
-        if (on) out = static_cast<T*>(p.out) + (tok * p.heads + w.kvh * p.group + r % p.group) * p.out_hd;
-        if (w.i > 0 || w.i1 < w.it.n)
-          part = p.part + (2ll * blockIdx.x + (w.i > 0 ? 0 : 1)) * paged_slot_floats<L::ROWS, HD>();
+        n_sink = g.n_sink;
+        w_shift = g.w_shift;
+        if (on)
+          out = static_cast<T*>(p.out) +
+                (static_cast<long long>(g.tok + h * half_tokens + t) * p.heads + g.kvh * p.group + row - t * p.group) *
+                    p.out_hd;
+        if (!g.whole) part = p.part + (2ll * blockIdx.x + (g.i0 > 0 ? 0 : 1)) * paged_slot_floats<L::ROWS, HD>();
       }
-      __syncwarp();  // read before lane 0 moves it on
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[L::B_GE + get.at]);
       if (last < 0) {  // nothing here for this half
         if (on && part) {
           part[L::ROWS * HD + item_row] = -INFINITY;
@@ -607,12 +640,11 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
       const int lo_pos = p.window > 0 ? pos - p.window + 1 : 0;
       const uint32_t tO = tS + L::TMEM_O + o_buf * HD;
       float m_run = -INFINITY, l_run = 0.f;
-      int prev = 0;  // ring position of the tile before
       bool first = true;
       for (;;) {
         const int k0 = (i < n_sink ? i : i + w_shift) * BN;
         const bool masked = k0 > k_hi || (k0 <= k_lo && k0 > k_sk);  // warp-uniform
-        if (!(ok = warp_wait_phase(&b[L::H_SF + s_buf], s_ph, wd, 0x542))) break;
+        if (!(ok = chunk_wait_warp(&b[L::H_SF + s_buf], s_ph, wd, 0x542))) break;
         tc_fence_after();
         const uint32_t tSb = tS + s_buf * BN;
         uint32_t sc[BN / 32][32];
@@ -644,9 +676,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
           a[10] = fmaxf(__uint_as_float(sc[g][30]), __uint_as_float(sc[g][31]));
           mg[g] = max3(max3(a[0], a[1], a[2]), max3(a[3], a[4], a[5]), max3(a[6], a[7], max3(a[8], a[9], a[10])));
         }
-        float m_tile = fmaxf(mg[0], mg[1]);
-        if constexpr (BN == 128) m_tile = fmaxf(m_tile, fmaxf(mg[2], mg[3]));
-        m_tile *= sl2;
+        const float m_tile = fmaxf(mg[0], mg[1]) * sl2;
         bool resc = false;
         float m_new = m_run;
         if (m_tile > m_run + 8.0f) {  // P stays below 2^8
@@ -655,8 +685,9 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         }
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
         if (__any_sync(~0u, resc)) {
-          // O must hold every earlier tile: P.V of the last one hands its stage back.
-          if (!(ok = warp_wait_phase(&bars[L::B_E + prev % NST], (prev / NST) & 1, wd, 0x543))) break;
+          // O must hold every earlier tile: wait for P.V of the last.
+          const int pb = s_buf == 0 ? NSB - 1 : s_buf - 1;
+          if (!(ok = chunk_wait_warp(&b[L::H_PE + pb], s_buf == 0 ? s_ph ^ 1 : s_ph, wd, 0x543))) break;
           tc_fence_after();
           const float corr = resc ? ex2_approx(m_run - m_new) : 1.f;
           l_run *= corr;
@@ -707,10 +738,8 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         }
         if (first && pend && !(ok = finish())) break;
         first = false;
-        prev = unit;
-        const int next = i + 1 >= range.a && i + 1 < range.c ? range.c : i + 1;
-        unit += next - i;
-        i = next;
+        ++i;
+        if (i >= a && i < c) i = c;
         if (i > last) break;
       }
       if (!ok) break;
@@ -733,7 +762,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == L::W_MMA) {
+  if (warp == L::W_S) {
     tc_fence_after();
     tmem_dealloc(tmem_base, L::TMEM_COLS);
   }
