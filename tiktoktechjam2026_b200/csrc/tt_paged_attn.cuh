@@ -171,28 +171,28 @@ struct PagedWalk {
   int end_b, end_kvh, end_qt, end_i;
   long long at, len;  // seek: where in the item the cut falls, and the item's length
 
+  // Places the walk on a cut.  The whole warp takes part: the item is found 32
+  // candidates at a time (this stands before a kernel's first load).
   __device__ __forceinline__ void seek(const PagedParams& p, const PagedCut& c, int tpi) {
+    const int lane = threadIdx.x & 31;
     b = c.b;
     s = paged_seq(p, b);
     nq = paged_q_tiles(p, s, tpi);
     const PagedLine<TK> line(p, s, nq, tpi);
     const long long head = line.all();
-    kvh = static_cast<int>(div_pos(c.off, head));
+    kvh = p.kv_heads == 1 ? 0 : static_cast<int>(div_pos(c.off, head));
     const long long off = c.off - kvh * head;
-    int lo = 0, hi = nq;  // the last item that begins at or before off
+    qt = 0;  // the last item that begins at or before off
     long long start = 0, next = head;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      const long long x = line.before(mid);
-      if (x <= off) {
-        lo = mid;
-        start = x;
-      } else {
-        hi = mid;
-        next = x;
-      }
+    for (int n = nq; n > 1;) {
+      const int step = (n + 31) >> 5, q = qt + lane * step;
+      const long long x = lane * step < n ? line.before(q) : head + 1;
+      const int hit = 31 - __clz(__ballot_sync(~0u, x <= off));  // (lane 0 always: q = qt)
+      start = __shfl_sync(~0u, x, hit);
+      if (hit < 31) next = min(next, __shfl_sync(~0u, x, hit + 1));
+      qt += hit * step;
+      n = min(step, n - hit * step);
     }
-    qt = lo;
     at = off - start;
     len = next - start;
     it.set(p, s, qt, tpi);
@@ -206,20 +206,14 @@ struct PagedWalk {
   }
 
   __device__ __forceinline__ bool at_end() const { return b == end_b && kvh == end_kvh && qt == end_qt; }
-  // Whether the piece from cut c to cut e holds any tile; places the walk on its first.
-  __device__ __forceinline__ bool begin(const PagedParams& p, const PagedCut& c, const PagedCut& e, int tpi) {
-    end_b = p.batch;
-    if (c.b < 0) return false;
-#pragma unroll 1
-    for (int k = e.b >= 0 ? 0 : 1; k < 2; ++k) {  // the end, then the beginning (one copy of the code)
-      seek(p, k == 0 ? e : c, tpi);
-      if (k == 0) {
-        end_b = b;
-        end_kvh = kvh;
-        end_qt = qt;
-        end_i = i;
-      }
-    }
+  __device__ __forceinline__ void end_at(const PagedWalk& e) {
+    end_b = e.b;
+    end_kvh = e.kvh;
+    end_qt = e.qt;
+    end_i = e.i;
+  }
+  // After seek and end_at: whether the piece holds any tile.
+  __device__ __forceinline__ bool begin() {
     i1 = at_end() ? end_i : it.n;
     return i < i1;
   }
@@ -285,12 +279,14 @@ __device__ __forceinline__ void paged_schedule(const PagedParams& p, int tpi, in
       __syncthreads();  // the round before has read warp_sum
       if (lane == 31) warp_sum[warp] = inc;
       __syncthreads();
-      long long before = carry;
-#pragma unroll 1
-      for (int w = 0; w < NWARPS; ++w) {
-        if (w == warp) before = carry;
-        carry += warp_sum[w];
+      long long sums = lane < NWARPS ? warp_sum[lane] : 0;
+#pragma unroll
+      for (int o = 1; o < NWARPS; o <<= 1) {
+        const long long v = __shfl_up_sync(~0u, sums, o);
+        if (lane >= o) sums += v;
       }
+      const long long before = carry + (warp > 0 ? __shfl_sync(~0u, sums, warp > 0 ? warp - 1 : 0) : 0);
+      carry += __shfl_sync(~0u, sums, NWARPS - 1);
       lo = before + inc - u;
       hi = before + inc;
       if (pass == 1) mark();
@@ -406,11 +402,15 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
   const int c = blockIdx.x + 1;  // worker 0 starts at an item's beginning
   paged_schedule<TK, 1, kJoinThreads>(p, tpi, min_tiles, c, &cut, &per);
   if (cut.b < 0) return;
-  if (threadIdx.x == 0) {
-    cur.seek(p, cut, tpi);
-    const bool mine = cur.i > 0 && cur.it.rows > static_cast<int>(blockIdx.y) * RB &&
-                      !(cur.at > per && cur.tile_at(cur.at - per) > 0);  // worker c - 1 starts inside too
-    n_after = mine ? static_cast<int>(div_pos(cur.len - cur.at + per - 1, per)) : 0;
+  if (threadIdx.x < 32) {
+    PagedWalk<TK> w;
+    w.seek(p, cut, tpi);
+    if (threadIdx.x == 0) {
+      cur = w;
+      const bool mine = cur.i > 0 && cur.it.rows > static_cast<int>(blockIdx.y) * RB &&
+                        !(cur.at > per && cur.tile_at(cur.at - per) > 0);  // worker c - 1 starts inside too
+      n_after = mine ? static_cast<int>(div_pos(cur.len - cur.at + per - 1, per)) : 0;
+    }
   }
   __syncthreads();
   if (n_after == 0) return;
@@ -519,9 +519,20 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
   paged_zero_outside(p, L::THREADS);
   pdl_trigger();
   const int worker = worker0 + warp;
-  PagedWalk<TK> cur, ahead;
-  if (!cur.begin(p, cuts[warp], cuts[warp + 1], tpi)) return;
-  ahead = cur;
+  // Each warp finds the cut at which its piece begins, the last one also the end of the block's pieces.
+  __shared__ PagedWalk<TK> found[L::WARPS + 1];
+  for (int w = warp; w <= L::WARPS; w += L::WARPS) {
+    PagedWalk<TK> x;
+    x.b = p.batch;
+    if (cuts[w].b >= 0) x.seek(p, cuts[w], tpi);
+    if (lane == 0) found[w] = x;
+  }
+  __syncthreads();
+  if (cuts[warp].b < 0) return;
+  PagedWalk<TK> cur = found[warp];
+  cur.end_at(found[warp + 1]);
+  if (!cur.begin()) return;
+  PagedWalk<TK> ahead = cur;
   bool more = true;  // `ahead` has a tile
 
   // Copies the K and V tile under `ahead` into stage st and moves it on.

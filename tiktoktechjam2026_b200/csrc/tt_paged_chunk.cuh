@@ -163,7 +163,7 @@ __device__ __forceinline__ void chunk_segment(const PagedParams& p, const PagedW
   g.w_shift = w.it.w_tile - w.it.n_sink;
   g.whole = w.i == 0 && w.i1 == w.it.n;
   g.kvh = w.kvh;
-  g.tok = w.s.q0 + w.it.r0 / p.group;
+  g.tok = w.s.q0 + w.qt * (L::NT * half_tokens);
   g.slot = w.s.slot;
   g.keys = w.s.L;
   // Only the item's last tile can hold the sequence's end.
@@ -173,12 +173,12 @@ __device__ __forceinline__ void chunk_segment(const PagedParams& p, const PagedW
   g.fix_at = r0 > 0 && r0 < BN && (r0 & (page - 1)) != 0 ? w.it.n - 1 : -1;
   for (int h = 0; h < L::NT; ++h) {
     ChunkHalf x = {};
-    const int hr = half_tokens * p.group;
-    x.rows = min(max(w.it.rows - h * hr, 0), hr);
+    const int tokens = min(max(w.it.p1 - w.it.p0 + 1 - h * half_tokens, 0), half_tokens);
+    x.rows = tokens * p.group;
     x.last = -1;
-    if (x.rows > 0) {
+    if (tokens > 0) {
       x.p0 = w.it.p0 + h * half_tokens;
-      x.p1 = x.p0 + (x.rows - 1) / p.group;
+      x.p1 = x.p0 + tokens - 1;
       const int end = x.p1 < 0 ? 0 : x.p1 / BN + 1;  // one past the last tile a row sees
       if (p.window == 0) {
         x.e = end;
@@ -235,25 +235,27 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   constexpr int BN = L::BN, NT = L::NT, NSB = L::NSB, NST = L::NST, NQ = L::NQ, NOB = L::NOB;
   extern __shared__ uint8_t smem_raw[];
   __shared__ PagedCut cuts[2];
-  __shared__ PagedWalk<BN> walk;  // the producer's
+  __shared__ PagedWalk<BN> walk, walk_end;  // the producer's piece
   __shared__ ChunkSegment segments[L::NSEG];
-  __shared__ bool any;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half_rows = half_tokens * p.group, tpi = NT * half_tokens;
   long long per;
   paged_schedule<BN, 2, L::THREADS>(p, tpi, min_tiles, blockIdx.x, cuts, &per);
   paged_zero_outside(p, L::THREADS);
   pdl_trigger();
-  if (threadIdx.x == 0) any = walk.begin(p, cuts[0], cuts[1], tpi);
-  __syncthreads();
-  if (!any) return;
-
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
-  if (threadIdx.x == 0) {
+  // The ends of the piece, the barriers and TMEM, each by a warp of its own.
+  if (warp < 2) {
+    PagedWalk<BN> x;
+    x.b = p.batch;
+    if (cuts[warp].b >= 0) x.seek(p, cuts[warp], tpi);
+    if (lane == 0) (warp == 0 ? walk : walk_end) = x;
+  }
+  if (threadIdx.x == 64) {
     for (int i = 0; i < NST; ++i) {
       mbar_init(&bars[L::B_F + i], 1);
       mbar_init(&bars[L::B_E + i], NT);
@@ -289,6 +291,11 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (threadIdx.x == 0 && cuts[0].b >= 0) {
+    walk.end_at(walk_end);
+    if (!walk.begin()) cuts[0].b = -1;
+  }
+  __syncthreads();
   const uint32_t tmem_base = *tmem_slot;
   const Watchdog wd{p.err, abort_flag, p.timeout_ns};
   const int page_rows = 1 << p.page_shift;
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     int u = 0, st = 0, nq[NT] = {};
     uint32_t ph = 0;
     Place put, get;
-    bool more = true;  // the walk stands on a segment that is not published yet
+    bool more = cuts[0].b >= 0;  // the walk stands on a segment that is not published yet
     bool ok = true;
     for (bool started = false;; started = true) {
       // Publishes the walk's segment (or the end) and moves the walk on.
@@ -536,6 +543,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     const int h = warp >> 2, q = warp & 3, row = q * 32 + lane;
     uint64_t* b = bars + L::B_HALF + h * L::N_HALF;
     const uint32_t tS = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * L::TMEM_HALF;
+    const int t = row / p.group;  // the row's token in the half
     const float sl2 = p.scale_log2;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
     bool ok = true;
@@ -611,7 +619,6 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         last = x.last;
         p0 = x.p0;
         p1 = x.p1;
-        const int t = row / p.group;
         pos = p0 + t;
         on = row < x.rows;
         n_sink = g.n_sink;
