@@ -96,11 +96,11 @@ int paged_workspace(int hd, int sm_count, size_t* bytes) {
   }
 }
 
-template <typename T, int HD, int TK, int ROWS, int RB>
+template <typename T, int HD, int TK, int ROWS, int RB, int THREADS>
 int launch_paged_join(const PagedParams& p, int tpi, int min_tiles, cudaStream_t stream) {
   if (p.n_workers > kPagedMaxWorkers) return fail(TT_ERR_UNSUPPORTED, "%d workers", p.n_workers);
   PdlScope programmatic;
-  launch_kernel(paged_join_kernel<T, HD, TK, ROWS, RB>, dim3(p.n_workers - 1, ROWS / RB), kJoinThreads, 0, stream, p,
+  launch_kernel(paged_join_kernel<T, HD, TK, ROWS, RB, THREADS>, dim3(p.n_workers - 1, ROWS / RB), THREADS, 0, stream, p,
                 tpi, min_tiles);
   return after_launch("paged attention join");
 }
@@ -116,7 +116,7 @@ int launch_paged_rows(PagedParams p, int row_lo, int row_hi, int sm_count, cudaS
   p.n_workers = sm_count * L::WARPS;
   launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, p, kRowsMax / p.group, kRowsMinTiles);
   if (int rc = after_launch("paged attention (rows)")) return rc;
-  return launch_paged_join<T, HD, L::TK, kRowsMax, kRowsMax>(p, kRowsMax / p.group, kRowsMinTiles, stream);
+  return launch_paged_join<T, HD, L::TK, kRowsMax, kRowsMax, 256>(p, kRowsMax / p.group, kRowsMinTiles, stream);
 }
 
 template <typename T, int HD>
@@ -147,7 +147,7 @@ int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t str
   }
   launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, tq, tk, tv, p, half_tokens, kChunkMinTiles);
   if (int rc = after_launch("paged attention (chunk)")) return rc;
-  return launch_paged_join<T, HD, L::BN, L::ROWS, 32>(p, L::NT * half_tokens, kChunkMinTiles, stream);
+  return launch_paged_join<T, HD, L::BN, L::ROWS, 32, 128>(p, L::NT * half_tokens, kChunkMinTiles, stream);
 }
 
 // Each sequence goes by its own number of query rows; max_rows only saves

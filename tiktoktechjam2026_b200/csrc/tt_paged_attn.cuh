@@ -374,7 +374,6 @@ __host__ __device__ constexpr long long paged_slot_floats() {
 // sums joined in a fixed order.  All blocks are resident at once, and most only
 // find that they have nothing to join: the schedule runs before the kernel
 // whose parts it reads has ended (programmatic launch).
-constexpr int kJoinThreads = 256;
 
 struct JoinSum {
   float m, l;
@@ -391,16 +390,16 @@ struct JoinSum {
   }
 };
 
-template <typename T, int HD, int TK, int ROWS, int RB>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedParams p, int tpi, int min_tiles) {
+template <typename T, int HD, int TK, int ROWS, int RB, int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_join_kernel(const PagedParams p, int tpi, int min_tiles) {
   __shared__ PagedCut cut;
   __shared__ uint8_t holds[kPagedMaxWorkers];  // whether the k-th worker from c on has a part
-  __shared__ JoinSum sums[kJoinThreads];
+  __shared__ JoinSum sums[THREADS];
   __shared__ PagedWalk<TK> cur;
   __shared__ int n_after;  // workers from c on that start inside the item; 0: nothing to join here
   long long per;
   const int c = blockIdx.x + 1;  // worker 0 starts at an item's beginning
-  paged_schedule<TK, 1, kJoinThreads>(p, tpi, min_tiles, c, &cut, &per);
+  paged_schedule<TK, 1, THREADS>(p, tpi, min_tiles, c, &cut, &per);
   if (cut.b < 0) return;
   if (threadIdx.x < 32) {
     PagedWalk<TK> w;
@@ -414,7 +413,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
   }
   __syncthreads();
   if (n_after == 0) return;
-  for (int k = threadIdx.x; k < n_after; k += kJoinThreads)
+  for (int k = threadIdx.x; k < n_after; k += THREADS)
     holds[k] = cur.tile_at(cur.at + k * per) < (k + 1 < n_after ? cur.tile_at(cur.at + (k + 1) * per) : cur.it.n);
   __syncthreads();
   pdl_wait();
@@ -422,25 +421,28 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
   constexpr long long SLOT = paged_slot_floats<ROWS, HD>();
   const float* first = p.part + (2ll * (c - 1) + 1) * SLOT;
   const float* rest = p.part + 2ll * c * SLOT;  // then every 2 SLOT
-  constexpr int TPR = HD / 4, GROUPS = kJoinThreads / TPR;
+  constexpr int TPR = HD / 4, GROUPS = THREADS / TPR;
   const int g = threadIdx.x / TPR, d = threadIdx.x % TPR * 4;
-  const int deal = rows < GROUPS ? GROUPS / rows : 1;  // threads over which a row's parts are dealt
+  // Rows of the block's threads, and the share of the parts that a thread takes.
+  const int deal = rows < GROUPS ? GROUPS / rows : 1;
+  const int share = deal > 1 ? g / rows : 0, row_in = deal > 1 ? g - share * rows : g;
   for (int r0 = 0; r0 < rows; r0 += GROUPS) {
-    const int row = row0 + r0 + g % min(rows, GROUPS), share = g / min(rows, GROUPS);
+    const int row = row0 + r0 + row_in;
     const bool on = row < row0 + rows && share < deal;
     JoinSum sum = {-INFINITY, 0.f, make_float4(0, 0, 0, 0)};
     if (on) {
       const int m_at = ROWS * HD + row, l_at = m_at + ROWS, o_at = row * HD + d;
-      if (share == 0) sum.add(first[m_at], first[l_at], *reinterpret_cast<const float4*>(first + o_at));
-      constexpr int U = 4;  // parts in flight
-      for (int k0 = share; k0 < n_after; k0 += U * deal) {
+      if (share == 0) sum = {first[m_at], first[l_at], *reinterpret_cast<const float4*>(first + o_at)};
+      int k = share;
+      constexpr int U = 4;  // parts in flight where they are many
+#pragma unroll 1
+      for (; k + (U - 1) * deal < n_after; k += U * deal) {
         float mk[U], lk[U];
         float4 ok[U];
 #pragma unroll
         for (int x = 0; x < U; ++x) {
-          const int k = k0 + x * deal;
-          const bool has = k < n_after && holds[k];
-          const float* s = rest + 2 * SLOT * (has ? k : 0);
+          const bool has = holds[k + x * deal];
+          const float* s = rest + 2 * SLOT * (k + x * deal);
           mk[x] = has ? s[m_at] : -INFINITY;
           lk[x] = has ? s[l_at] : 0.f;
           ok[x] = has ? *reinterpret_cast<const float4*>(s + o_at) : make_float4(0, 0, 0, 0);
@@ -448,6 +450,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
 #pragma unroll
         for (int x = 0; x < U; ++x) sum.add(mk[x], lk[x], ok[x]);
       }
+#pragma unroll 1
+      for (; k < n_after; k += deal)
+        if (holds[k]) {
+          const float* s = rest + 2 * SLOT * k;
+          sum.add(s[m_at], s[l_at], *reinterpret_cast<const float4*>(s + o_at));
+        }
     }
     if (deal > 1) {
       sums[threadIdx.x] = sum;
@@ -460,7 +468,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
     }
     if (on && share == 0 && d < p.out_hd) {
       const float inv = sum.l > 0.f ? 1.f / sum.l : 0.f;
-      const int r = cur.it.r0 + row, tok = cur.s.q0 + r / p.group, h = cur.kvh * p.group + r % p.group;
+      const int t = row / p.group, tok = cur.s.q0 + cur.qt * tpi + t, h = cur.kvh * p.group + row - t * p.group;
       uint2* dst = reinterpret_cast<uint2*>(static_cast<T*>(p.out) +
                                             (static_cast<long long>(tok) * p.heads + h) * p.out_hd + d);
       *dst = make_uint2(Pair16<T>::pack(sum.o.x * inv, sum.o.y * inv), Pair16<T>::pack(sum.o.z * inv, sum.o.w * inv));
@@ -494,6 +502,18 @@ struct PagedRowsLayout {
   static constexpr int SWM = CH < 8 ? CH - 1 : 7;
   static_assert(SMEM <= 232448, "shared memory budget");
 };
+
+// 16-byte asynchronous copy of data that is read once (first to leave L2).
+__device__ __forceinline__ uint64_t policy_evict_first() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void cp_async_16_once(uint32_t dst, const void* src, uint32_t src_bytes, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(src_bytes),
+               "l"(policy)
+               : "memory");
+}
 
 // Byte offset of 16-byte piece c of row r: the pieces are permuted so that the
 // same piece of eight consecutive rows falls into eight different bank groups.
@@ -534,6 +554,7 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
   if (!cur.begin()) return;
   PagedWalk<TK> ahead = cur;
   bool more = true;  // `ahead` has a tile
+  const uint64_t policy = policy_evict_first();
 
   // Copies the K and V tile under `ahead` into stage st and moves it on.
   auto fetch = [&](int st) {
@@ -552,10 +573,10 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
       const long long in_page =
           (static_cast<long long>(ahead.kvh) << p.page_shift) * HD + (key & ((1 << p.page_shift) - 1)) * HD + ch * 8;
       const long long at = ok ? pg : 0;
-      cp_async_16(sk + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.k_pages) + at * p.k_stride + in_page,
-                  ok ? 16u : 0u);
-      cp_async_16(sv + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.v_pages) + at * p.v_stride + in_page,
-                  ok ? 16u : 0u);
+      cp_async_16_once(sk + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.k_pages) + at * p.k_stride + in_page,
+                       ok ? 16u : 0u, policy);
+      cp_async_16_once(sv + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.v_pages) + at * p.v_stride + in_page,
+                       ok ? 16u : 0u, policy);
     }
     if (++ahead.i == ahead.i1) more = ahead.next(p, tpi);
   };
