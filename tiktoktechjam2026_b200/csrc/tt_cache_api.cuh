@@ -76,6 +76,11 @@ constexpr int kRowsMax = 16;
 // Key tiles that a worker takes at least: shorter pieces would cost more in
 // joining than they save.
 constexpr int kRowsMinTiles = 2, kChunkMinTiles = 4;
+// What an item costs beside its key tiles (its queries, its output, the
+// pipeline's run in and out), in tiles.  Ragged chunks over 8K caches, 424 items:
+// 334 us with 2 for the chunk kernel, 300 with 4, 290 with 6, 294 with 12;
+// calls whose items are alike do not depend on it.
+constexpr int kRowsItemTiles = 3, kChunkItemTiles = 6;
 
 template <int HD>
 size_t paged_part_bytes(int sm_count) {
@@ -114,6 +119,7 @@ int launch_paged_rows(PagedParams p, int row_lo, int row_hi, int sm_count, cudaS
   p.row_lo = row_lo;
   p.row_hi = row_hi;
   p.n_workers = sm_count * L::WARPS;
+  p.item_len = kRowsItemTiles * L::TK;
   launch_kernel(kern, sm_count, L::THREADS, L::SMEM, stream, p, kRowsMax / p.group, kRowsMinTiles);
   if (int rc = after_launch("paged attention (rows)")) return rc;
   return launch_paged_join<T, HD, L::TK, kRowsMax, kRowsMax, 256>(p, kRowsMax / p.group, kRowsMinTiles, stream);
@@ -131,6 +137,7 @@ int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t str
   p.row_lo = row_lo;
   p.row_hi = 0x7fffffff;
   p.n_workers = sm_count;
+  p.item_len = kChunkItemTiles * L::BN;
   const int half_tokens = 128 / p.group, page = 1 << p.page_shift;
   CUtensorMap tq, tk, tv;
   {
@@ -156,8 +163,8 @@ template <typename T, int HD>
 int launch_paged(const PagedParams& p, int max_rows, int sm_count, cudaStream_t stream) {
   if (max_rows <= kRowsMax) return launch_paged_rows<T, HD>(p, 0, 0x7fffffff, sm_count, stream);
   // With few (sequence, KV head) pairs the chunk kernel takes short sequences
-  // along, at most two per SM: that costs less than a second pair of launches
-  // (SEE_LOG).
+  // along, at most two per SM: a second pair of launches that finds no short
+  // sequence costs 8 us.
   if (p.group > kRowsMax || static_cast<long long>(p.batch) * p.kv_heads <= 2ll * sm_count)
     return launch_paged_chunk<T, HD>(p, 0, sm_count, stream);
   if (int rc = launch_paged_chunk<T, HD>(p, kRowsMax + 1, sm_count, stream)) return rc;

@@ -45,6 +45,7 @@ struct PagedParams {
   int out_hd;
   int row_lo, row_hi;          // this launch serves sequences of row_lo .. row_hi query rows (T * group)
   int n_workers;
+  int item_len;                // extra length of an item on the line, in keys: its queries' loads and its output
   float scale_log2;
   unsigned int* err;
   unsigned long long timeout_ns;
@@ -70,9 +71,6 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
 }
 
 constexpr int kPagedMaxWorkers = 2048;
-
-// Extra length of an item on the line, in key tiles: its queries' loads and its output.
-constexpr int kPagedItemTiles = 2;
 
 // One item: the tokens qt * tpi .. of a sequence (rows: token * group + head of
 // the group) and the key tiles that some row of it can see.  With a window the
@@ -135,10 +133,10 @@ __device__ __forceinline__ int ramp_start(long long a, int d) {
 template <int TK>
 struct PagedLine {
   long long up, gap;  // p1(0) + 1; p0(0) + 1 - window - sinks
-  int up0, gap0, nq, tpi, L;
+  int up0, gap0, nq, tpi, L, item_len;
   bool window;
   __device__ __forceinline__ PagedLine(const PagedParams& p, const PagedSeq& s, int nq_, int tpi_)
-      : nq(nq_), tpi(tpi_), L(s.L), window(p.window > 0) {
+      : nq(nq_), tpi(tpi_), L(s.L), item_len(p.item_len), window(p.window > 0) {
     const long long base = s.L - s.T;
     up = base + tpi;
     up0 = ramp_start(up, tpi);
@@ -148,7 +146,7 @@ struct PagedLine {
   __device__ __forceinline__ long long before(int q) const {
     if (q == 0) return 0;
     const int whole = q == nq ? q - 1 : q;  // the last item may hold fewer tokens
-    long long len = static_cast<long long>(q) * (kPagedItemTiles * TK) + ramp_sum(up, tpi, up0, whole);
+    long long len = static_cast<long long>(q) * item_len + ramp_sum(up, tpi, up0, whole);
     if (q == nq) len += L;
     if (window) len -= ramp_sum(gap, tpi, gap0, q);
     return len;

@@ -10,7 +10,7 @@ compose the ops themselves; the model path calls ``tt_model_forward`` once.
 
 from __future__ import annotations
 
-from ctypes import c_int64, c_size_t
+from ctypes import byref, c_int64, c_size_t
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -241,14 +241,16 @@ def _cache(k: Optional[torch.Tensor], v: Optional[torch.Tensor], tables: torch.T
                    layers, pages, kv_heads, page, head_dim, slots, width)
 
 
-def _run(device: int, fn, *args) -> None:
+def _run(device: int, fn, cache: KVCache, *args) -> None:
     """Calls a libtt_b200 entry point on the device's current stream."""
     stream = torch.cuda.current_stream(device).cuda_stream
     if torch.cuda.current_device() == device:
-        check(fn(*args, stream))
-        return
-    with torch.cuda.device(device):
-        check(fn(*args, stream))
+        rc = fn(byref(cache), *args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(byref(cache), *args, stream)
+    if rc:
+        check(rc)
 
 
 def _batch(cu_q: torch.Tensor, slots: Optional[torch.Tensor], tables: torch.Tensor) -> Tuple[int, int, int]:
@@ -278,8 +280,7 @@ def cache_reserve(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, 
     return status
 
 
-def _token_strides(t: torch.Tensor):
-    return (c_int64 * 3)(*t.stride())
+_Strides = c_int64 * 3
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
@@ -300,7 +301,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if k.dtype is not k_pages.dtype or v.dtype is not k_pages.dtype or k.get_device() != dev or v.get_device() != dev:
         raise ValueError("k and v must have the pages' dtype and device")
     cu, sl, n = _batch(cu_q, slots, tables)
-    _run(tables.get_device(), lib().tt_cache_append, c, k.data_ptr(), _token_strides(k), v.data_ptr(), _token_strides(v),
+    _run(tables.get_device(), lib().tt_cache_append, c, k.data_ptr(), _Strides(*k.stride()), v.data_ptr(), _Strides(*v.stride()),
          want[0], cu, sl, n, _index(status, "status", dev))
 
 
