@@ -125,6 +125,18 @@ int launch_paged_rows(PagedParams p, int row_lo, int row_hi, int sm_count, cudaS
   return launch_paged_join<T, HD, L::TK, kRowsMax, kRowsMax, 256>(p, kRowsMax / p.group, kRowsMinTiles, stream);
 }
 
+// Cache that one block of the kernel without cuts may have to stream: at more,
+// a lone long sequence would take longer on its block than cut over the GPU.
+constexpr long long kItemBytes = 640 * 1024;
+
+template <typename T, int HD>
+int launch_paged_item(const PagedParams& p, cudaStream_t stream) {
+  auto kern = paged_item_kernel<T, HD>;
+  if (int rc = prepare_kernel(kern, kItemSmem<HD>)) return rc;
+  launch_kernel(kern, dim3(p.kv_heads, p.batch), 32 * kItemWarps, kItemSmem<HD>, stream, p, kRowsMax / p.group);
+  return after_launch("paged attention (items)");
+}
+
 template <typename T, int HD>
 int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t stream) {
   using L = PagedChunkLayout<HD>;
@@ -161,6 +173,12 @@ int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t str
 // launches whose kernel could have no work.
 template <typename T, int HD>
 int launch_paged(const PagedParams& p, int max_rows, int sm_count, cudaStream_t stream) {
+  if (max_rows <= kRowsMax) {
+    const long long room = static_cast<long long>(p.table_width) << p.page_shift;
+    const long long reach = static_cast<long long>(p.window) + p.sinks + kRowsMax;  // keys that a window leaves an item
+    const long long keys = p.window > 0 && reach < room ? reach : room;
+    if (p.batch > 0 && p.batch <= 65535 && keys * HD * 4 <= kItemBytes) return launch_paged_item<T, HD>(p, stream);
+  }
   if (max_rows <= kRowsMax) return launch_paged_rows<T, HD>(p, 0, 0x7fffffff, sm_count, stream);
   // With few (sequence, KV head) pairs the chunk kernel takes short sequences
   // along, at most two per SM: a second pair of launches that finds no short

@@ -521,6 +521,171 @@ __device__ __forceinline__ uint32_t paged_rows_at(int r, int c) {
   return r * L::RB + ((c ^ ((r / L::RPL) & L::SWM)) << 4);
 }
 
+// Copies keys k0 .. k0 + TK - 1 of one KV head and their values to sk (then the values).
+template <typename T, int HD>
+__device__ __forceinline__ void paged_rows_fetch(const PagedParams& p, const int* row, int n_keys, int kvh, int k0,
+                                                 uint32_t sk, uint64_t policy) {
+  using L = PagedRowsLayout<HD>;
+  const int lane = threadIdx.x & 31;
+  const int page_at = (k0 >> p.page_shift) + lane;
+  int page = page_at < p.table_width ? row[page_at] : -1;  // lane i: the i-th page of the tile
+  if (page >= p.n_pages) page = -1;
+  const uint32_t sv = sk + L::TILE;
+#pragma unroll
+  for (int c0 = 0; c0 < L::TK * L::CH; c0 += 32) {
+    const int c = c0 + lane, r = c / L::CH, ch = c % L::CH;
+    const int key = k0 + r;
+    const int pg = __shfl_sync(~0u, page, (key >> p.page_shift) - (k0 >> p.page_shift));
+    const bool ok = pg >= 0 && key < n_keys;
+    const long long in_page =
+        (static_cast<long long>(kvh) << p.page_shift) * HD + (key & ((1 << p.page_shift) - 1)) * HD + ch * 8;
+    const long long at = ok ? pg : 0;
+    cp_async_16_once(sk + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.k_pages) + at * p.k_stride + in_page,
+                     ok ? 16u : 0u, policy);
+    cp_async_16_once(sv + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.v_pages) + at * p.v_stride + in_page,
+                     ok ? 16u : 0u, policy);
+  }
+}
+
+// A warp's softmax over the tiles that it takes of an item: queries, running
+// maximum and sum (this lane's keys) and O, as fragments of the MMA; a lane has
+// rows lane / 4 and lane / 4 + 8.
+template <typename T, int HD>
+struct PagedRows {
+  using L = PagedRowsLayout<HD>;
+  using PT = Pair16<T>;
+  static constexpr int TK = L::TK;
+  uint32_t qf[HD / 16][4];
+  float o[HD / 8][4];
+  float m[2], l[2];
+  int pos[2];
+
+  __device__ __forceinline__ void start(const PagedParams& p, const PagedSeq& seq, const PagedItem<TK>& it, int kvh) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = min(lane / 4 + 8 * h, it.rows - 1) + it.r0;
+            const int tok = r / p.group, head = kvh * p.group + r % p.group;
+            pos[h] = seq.L - seq.T + tok;
+            const T* src = static_cast<const T*>(p.q) + (seq.q0 + tok) * p.q_token + head * p.q_head + lane % 4 * 2;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              qf[kk][h] = *reinterpret_cast<const uint32_t*>(src + kk * 16);
+              qf[kk][2 + h] = *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8);
+            }
+            m[h] = -INFINITY;
+            l[h] = 0.f;
+          }
+#pragma unroll
+          for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+  }
+
+  __device__ __forceinline__ void tile(const PagedParams& p, uint32_t sk, int k0, bool whole) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t sv = sk + L::TILE;
+        float s[TK / 8][4];
+#pragma unroll
+        for (int n = 0; n < TK / 8; n += 2) {
+          float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            uint32_t b[4];  // keys 8n .. 8n+7 at features 0-7, 8-15, then keys 8n+8 .. 8n+15
+            ldmatrix_x4(sk + paged_rows_at<HD>(8 * n + (lane & 7) + (lane & 16 ? 8 : 0), 2 * kk + ((lane >> 3) & 1)), b);
+            PT::mma(s0, qf[kk], b[0], b[1]);
+            PT::mma(s1, qf[kk], b[2], b[3]);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            s[n][x] = s0[x] * p.scale_log2;
+            s[n + 1][x] = s1[x] * p.scale_log2;
+          }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int n = 0; n < TK / 8; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int key = k0 + 8 * n + lane % 4 * 2 + (x & 1), t = pos[x >> 1];
+              if (key > t || (p.window > 0 && t - key >= p.window && key >= p.sinks)) s[n][x] = -INFINITY;
+            }
+        }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < TK / 8; ++n) {
+          top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
+          top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]));
+        }
+        float base[2];
+        bool moved = false;
+        float corr[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
+          top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
+          const float next = fmaxf(m[h], top[h]);
+          base[h] = next == -INFINITY ? 0.f : next;  // a row that has seen no key: every 2^(s - 0) below is 0
+          corr[h] = ex2_approx(m[h] - base[h]);
+          moved |= next > m[h];
+          m[h] = next;
+          l[h] *= corr[h];
+        }
+        if (__any_sync(~0u, moved)) {
+#pragma unroll
+          for (int d = 0; d < HD / 8; ++d) {
+            o[d][0] *= corr[0];
+            o[d][1] *= corr[0];
+            o[d][2] *= corr[1];
+            o[d][3] *= corr[1];
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < TK / 8; n += 2) {
+          uint32_t pf[4];
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float e0 = ex2_approx(s[n + g][0] - base[0]), e1 = ex2_approx(s[n + g][1] - base[0]);
+            const float e2 = ex2_approx(s[n + g][2] - base[1]), e3 = ex2_approx(s[n + g][3] - base[1]);
+            l[0] += e0 + e1;
+            l[1] += e2 + e3;
+            pf[2 * g] = PT::pack(e0, e1);
+            pf[2 * g + 1] = PT::pack(e2, e3);
+          }
+#pragma unroll
+          for (int d = 0; d < HD / 8; d += 2) {
+            uint32_t b[4];  // keys 8n .. 8n+15 (two halves) at features 8d .. 8d+7, then the next eight
+            ldmatrix_x4_trans(sv + paged_rows_at<HD>(8 * n + (lane & 15), d + (lane >> 4)), b);
+            PT::mma(o[d], pf, b[0], b[1]);
+            PT::mma(o[d + 1], pf, b[2], b[3]);
+          }
+        }
+  }
+
+  // Makes l the sums of whole rows.
+  __device__ __forceinline__ void close() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(~0u, l[h], 1);
+      l[h] += __shfl_xor_sync(~0u, l[h], 2);
+    }
+  }
+  // Leaves the part (O unnormalised, m, l) at `slot`, laid out for 16 rows.
+  __device__ __forceinline__ void leave(float* slot, int rows) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = lane / 4 + 8 * h;
+      if (row >= rows) continue;
+      if (lane % 4 == 0) {
+        slot[16 * HD + row] = m[h];
+        slot[16 * HD + 16 + row] = l[h];
+      }
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d)
+        *reinterpret_cast<float2*>(slot + row * HD + 8 * d + lane % 4 * 2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+    }
+  }
+};
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
     paged_rows_kernel(const PagedParams p, int tpi, int min_tiles) {
@@ -556,26 +721,8 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
 
   // Copies the K and V tile under `ahead` into stage st and moves it on.
   auto fetch = [&](int st) {
-    const int k0 = ahead.it.tile(ahead.i) * TK;
-    const int* row = p.tables + ahead.s.slot * p.table_stride;
-    const int page_at = (k0 >> p.page_shift) + lane;
-    int page = page_at < p.table_width ? row[page_at] : -1;  // lane i: the i-th page of the tile
-    if (page >= p.n_pages) page = -1;
-    const uint32_t sk = ring + st * L::STAGE, sv = sk + L::TILE;
-#pragma unroll
-    for (int c0 = 0; c0 < TK * L::CH; c0 += 32) {
-      const int c = c0 + lane, r = c / L::CH, ch = c % L::CH;
-      const int key = k0 + r;
-      const int pg = __shfl_sync(~0u, page, (key >> p.page_shift) - (k0 >> p.page_shift));
-      const bool ok = pg >= 0 && key < ahead.s.L;
-      const long long in_page =
-          (static_cast<long long>(ahead.kvh) << p.page_shift) * HD + (key & ((1 << p.page_shift) - 1)) * HD + ch * 8;
-      const long long at = ok ? pg : 0;
-      cp_async_16_once(sk + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.k_pages) + at * p.k_stride + in_page,
-                       ok ? 16u : 0u, policy);
-      cp_async_16_once(sv + paged_rows_at<HD>(r, ch), static_cast<const T*>(p.v_pages) + at * p.v_stride + in_page,
-                       ok ? 16u : 0u, policy);
-    }
+    paged_rows_fetch<T, HD>(p, p.tables + ahead.s.slot * p.table_stride, ahead.s.L, ahead.kvh,
+                            ahead.it.tile(ahead.i) * TK, ring + st * L::STAGE, policy);
     if (++ahead.i == ahead.i1) more = ahead.next(p, tpi);
   };
 
@@ -585,154 +732,42 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
     cp_async_commit();
   }
 
-  uint32_t qf[HD / 16][4];
-  float o[HD / 8][4];
-  float m[2], l[2];
-  int pos[2];
+  PagedRows<T, HD> x;
   bool fresh = true;
   bool from_start = cur.i == 0;  // the current item's first tile is in this piece
   int st = 0;
   for (;;) {
     if (fresh) {
       fresh = false;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = min(lane / 4 + 8 * h, cur.it.rows - 1) + cur.it.r0;
-        const int tok = r / p.group, head = cur.kvh * p.group + r % p.group;
-        pos[h] = cur.s.L - cur.s.T + tok;
-        const T* src = static_cast<const T*>(p.q) + (cur.s.q0 + tok) * p.q_token + head * p.q_head + lane % 4 * 2;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          qf[kk][h] = *reinterpret_cast<const uint32_t*>(src + kk * 16);
-          qf[kk][2 + h] = *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8);
-        }
-        m[h] = -INFINITY;
-        l[h] = 0.f;
-      }
-#pragma unroll
-      for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+      x.start(p, cur.s, cur.it, cur.kvh);
     }
     if (more) fetch(st == 0 ? NST - 1 : st - 1);
     cp_async_commit();
     cp_async_wait<NST - 1>();
     __syncwarp();
-    const uint32_t sk = ring + st * L::STAGE, sv = sk + L::TILE;
+    const uint32_t sk = ring + st * L::STAGE;
     if (++st == NST) st = 0;
     const int k0 = cur.it.tile(cur.i) * TK;
-    const bool whole = cur.it.whole(p, k0);
-
-    float s[TK / 8][4];
-#pragma unroll
-    for (int n = 0; n < TK / 8; n += 2) {
-      float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk) {
-        uint32_t b[4];  // keys 8n .. 8n+7 at features 0-7, 8-15, then keys 8n+8 .. 8n+15
-        ldmatrix_x4(sk + paged_rows_at<HD>(8 * n + (lane & 7) + (lane & 16 ? 8 : 0), 2 * kk + ((lane >> 3) & 1)), b);
-        PT::mma(s0, qf[kk], b[0], b[1]);
-        PT::mma(s1, qf[kk], b[2], b[3]);
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        s[n][x] = s0[x] * p.scale_log2;
-        s[n + 1][x] = s1[x] * p.scale_log2;
-      }
-    }
-    if (!whole) {
-#pragma unroll
-      for (int n = 0; n < TK / 8; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int key = k0 + 8 * n + lane % 4 * 2 + (x & 1), t = pos[x >> 1];
-          if (key > t || (p.window > 0 && t - key >= p.window && key >= p.sinks)) s[n][x] = -INFINITY;
-        }
-    }
-    float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int n = 0; n < TK / 8; ++n) {
-      top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
-      top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]));
-    }
-    float base[2];
-    bool moved = false;
-    float corr[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
-      const float next = fmaxf(m[h], top[h]);
-      base[h] = next == -INFINITY ? 0.f : next;  // a row that has seen no key: every 2^(s - 0) below is 0
-      corr[h] = ex2_approx(m[h] - base[h]);
-      moved |= next > m[h];
-      m[h] = next;
-      l[h] *= corr[h];
-    }
-    if (__any_sync(~0u, moved)) {
-#pragma unroll
-      for (int d = 0; d < HD / 8; ++d) {
-        o[d][0] *= corr[0];
-        o[d][1] *= corr[0];
-        o[d][2] *= corr[1];
-        o[d][3] *= corr[1];
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < TK / 8; n += 2) {
-      uint32_t pf[4];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const float e0 = ex2_approx(s[n + g][0] - base[0]), e1 = ex2_approx(s[n + g][1] - base[0]);
-        const float e2 = ex2_approx(s[n + g][2] - base[1]), e3 = ex2_approx(s[n + g][3] - base[1]);
-        l[0] += e0 + e1;
-        l[1] += e2 + e3;
-        pf[2 * g] = PT::pack(e0, e1);
-        pf[2 * g + 1] = PT::pack(e2, e3);
-      }
-#pragma unroll
-      for (int d = 0; d < HD / 8; d += 2) {
-        uint32_t b[4];  // keys 8n .. 8n+15 (two halves) at features 8d .. 8d+7, then the next eight
-        ldmatrix_x4_trans(sv + paged_rows_at<HD>(8 * n + (lane & 15), d + (lane >> 4)), b);
-        PT::mma(o[d], pf, b[0], b[1]);
-        PT::mma(o[d + 1], pf, b[2], b[3]);
-      }
-    }
+    x.tile(p, sk, k0, cur.it.whole(p, k0));
     __syncwarp();  // every lane has read the stage before a later round refills it
 
     if (++cur.i == cur.i1) {  // the item, or its part in this piece, is done
-      const bool last = cur.i1 == cur.it.n;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(~0u, l[h], 1);
-        l[h] += __shfl_xor_sync(~0u, l[h], 2);
-      }
-      if (last && from_start) {
+      x.close();
+      if (cur.i1 == cur.it.n && from_start) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int row = lane / 4 + 8 * h;
           if (row >= cur.it.rows) continue;
-          const float inv = l[h] > 0.f ? 1.f / l[h] : 0.f;
+          const float inv = x.l[h] > 0.f ? 1.f / x.l[h] : 0.f;
           const int r = cur.it.r0 + row, tok = cur.s.q0 + r / p.group, head = cur.kvh * p.group + r % p.group;
           T* dst = static_cast<T*>(p.out) + (static_cast<long long>(tok) * p.heads + head) * p.out_hd + lane % 4 * 2;
 #pragma unroll
           for (int d = 0; d < HD / 8; ++d)
             if (8 * d < p.out_hd)
-              *reinterpret_cast<uint32_t*>(dst + 8 * d) = PT::pack(o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
+              *reinterpret_cast<uint32_t*>(dst + 8 * d) = PT::pack(x.o[d][2 * h] * inv, x.o[d][2 * h + 1] * inv);
         }
       } else {
-        float* slot = p.part + (2ll * worker + (from_start ? 1 : 0)) * paged_slot_floats<16, HD>();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = lane / 4 + 8 * h;
-          if (row >= cur.it.rows) continue;
-          if (lane % 4 == 0) {
-            slot[16 * HD + row] = m[h];
-            slot[16 * HD + 16 + row] = l[h];
-          }
-#pragma unroll
-          for (int d = 0; d < HD / 8; ++d)
-            *reinterpret_cast<float2*>(slot + row * HD + 8 * d + lane % 4 * 2) =
-                make_float2(o[d][2 * h], o[d][2 * h + 1]);
-        }
+        x.leave(p.part + (2ll * worker + (from_start ? 1 : 0)) * paged_slot_floats<16, HD>(), cur.it.rows);
       }
       fresh = true;
       from_start = true;
@@ -740,6 +775,85 @@ __global__ void __launch_bounds__(PagedRowsLayout<HD>::THREADS, 1)
     }
   }
   cp_async_wait<0>();
+}
+
+// Short chunks over short caches: one block per sequence and KV head, whose
+// warps take the item's tiles in turn and join their parts in shared memory.
+// No schedule and no second kernel, so the call is as short as its chain of
+// loads (lengths, page numbers, keys); a long cache would leave the GPU to a
+// few blocks.  One token over 1001 keys, 8 heads of 32: ITEM_LOG.
+constexpr int kItemWarps = 4;
+template <int HD>
+constexpr int kItemSmem = kItemWarps * PagedRowsLayout<HD>::NST * PagedRowsLayout<HD>::STAGE + 128;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(32 * kItemWarps) paged_item_kernel(const PagedParams p, int tpi) {
+  using L = PagedRowsLayout<HD>;
+  constexpr int TK = L::TK, NST = L::NST, THREADS = 32 * kItemWarps;
+  constexpr int SLOT = static_cast<int>(paged_slot_floats<16, HD>());
+  static_assert(kItemWarps * SLOT * 4 + 128 <= kItemSmem<HD>, "the parts take the ring's place");
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
+  const uint32_t ring = smem_u32(smem) + warp * NST * L::STAGE;
+  float* parts = reinterpret_cast<float*>(smem);
+  const int kvh = blockIdx.x, b = blockIdx.y;
+  const PagedSeq s = paged_seq(p, b);
+  if (kvh == 0 && b == 0) {  // rows of no sequence
+    const int lo = min(max(p.cu_q[0], 0), p.n_tokens), hi = min(max(p.cu_q[p.batch], lo), p.n_tokens);
+    const long long row = static_cast<long long>(p.heads) * p.out_hd / 8, n = (lo + p.n_tokens - hi) * row;
+    for (long long i = threadIdx.x; i < n; i += THREADS)
+      static_cast<uint4*>(p.out)[i < lo * row ? i : i - lo * row + hi * row] = make_uint4(0, 0, 0, 0);
+  }
+  const int* row = p.tables + s.slot * p.table_stride;
+  const uint64_t policy = policy_evict_first();
+  PagedItem<TK> it;
+  for (int qt = 0; qt * tpi < s.T; ++qt) {
+    it.set(p, s, qt, tpi);
+    int ahead = warp;
+#pragma unroll
+    for (int st = 0; st < NST - 1; ++st, ahead += kItemWarps) {
+      if (ahead < it.n) paged_rows_fetch<T, HD>(p, row, s.L, kvh, it.tile(ahead) * TK, ring + st * L::STAGE, policy);
+      cp_async_commit();
+    }
+    PagedRows<T, HD> x;
+    x.start(p, s, it, kvh);
+    int st = 0;
+#pragma unroll 1
+    for (int i = warp; i < it.n; i += kItemWarps, ahead += kItemWarps) {
+      if (ahead < it.n)
+        paged_rows_fetch<T, HD>(p, row, s.L, kvh, it.tile(ahead) * TK, ring + (st == 0 ? NST - 1 : st - 1) * L::STAGE,
+                                policy);
+      cp_async_commit();
+      cp_async_wait<NST - 1>();
+      __syncwarp();
+      const int k0 = it.tile(i) * TK;
+      x.tile(p, ring + st * L::STAGE, k0, it.whole(p, k0));
+      if (++st == NST) st = 0;
+      __syncwarp();  // every lane has read the stage before a later round refills it
+    }
+    x.close();
+    cp_async_wait<0>();
+    __syncthreads();  // every ring is done with
+    x.leave(parts + warp * SLOT, it.rows);
+    __syncthreads();
+    constexpr int TPR = HD / 4;
+    for (int y = threadIdx.x; y < it.rows * TPR; y += THREADS) {
+      const int r = y / TPR, d = y % TPR * 4;
+      JoinSum sum = {parts[16 * HD + r], parts[16 * HD + 16 + r], *reinterpret_cast<const float4*>(parts + r * HD + d)};
+#pragma unroll
+      for (int w = 1; w < kItemWarps; ++w) {
+        const float* q = parts + w * SLOT;
+        sum.add(q[16 * HD + r], q[16 * HD + 16 + r], *reinterpret_cast<const float4*>(q + r * HD + d));
+      }
+      if (d >= p.out_hd) continue;
+      const float inv = sum.l > 0.f ? 1.f / sum.l : 0.f;
+      const int t = r / p.group, tok = s.q0 + qt * tpi + t, head = kvh * p.group + r - t * p.group;
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (static_cast<long long>(tok) * p.heads + head) * p.out_hd + d) =
+          make_uint2(Pair16<T>::pack(sum.o.x * inv, sum.o.y * inv), Pair16<T>::pack(sum.o.z * inv, sum.o.w * inv));
+    }
+    __syncthreads();  // before the next item's copies
+  }
 }
 
 }  // namespace tt
