@@ -272,8 +272,11 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
                        size_t workspace_bytes, void* stream);
 
 /* Workspace bytes that tt_paged_attention needs on the current device for
- * these heads, whatever the batch and the lengths. */
+ * these heads, whatever the lengths; 0 (workspace may be NULL) where max_q_len
+ * (<= 0: not known), window, sinks, table_width and page keep every item so
+ * short that none is cut and the batch is below 65536. */
 int tt_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int max_q_len,
+                                       int window, int sinks, int table_width, int page,
                                        size_t* bytes);
 
 /* ---- whole model ----------------------------------------------------------- */

@@ -582,14 +582,17 @@ def test_refusals(tt_lib):
 
 @gpu
 def test_workspace_too_small_is_refused(tt_lib):
-    book = Book(1, [20], 2, 32, 16, torch.float16)
-    q = torch.randn(1, 2, 32, device=DEV).half()
-    out = torch.zeros(1, 64, dtype=torch.float16, device=DEV)
-    c = ops._cache(book.pages_k, book.pages_v, book.tables, book.lens, None)
-    ws = torch.empty(64, dtype=torch.uint8, device=DEV)
-    rc = tt_lib.tt_paged_attention(c, q.data_ptr(), 64, 32, ints([0, 1]).data_ptr(), 0, 1, out.data_ptr(), 1, 2, 32, 0,
-                                   1.0, 0, 0, 1, ws.data_ptr(), 64, 0)
-    assert rc == _lib.TT_ERR_WORKSPACE and torch.all(out == 0)
+    """Calls that may cut an item need their workspace; one that cannot takes none."""
+    for total, rc_want in ((6000, _lib.TT_ERR_WORKSPACE), (20, _lib.TT_OK)):
+        book = Book(1, [total], 2, 32, 16, torch.float16)
+        q = torch.randn(1, 2, 32, device=DEV).half()
+        out = torch.zeros(1, 64, dtype=torch.float16, device=DEV)
+        c = ops._cache(book.pages_k, book.pages_v, book.tables, book.lens, None)
+        ws = torch.empty(64, dtype=torch.uint8, device=DEV)
+        for ptr, size in ((ws.data_ptr(), 64), (None, 1 << 40)):
+            rc = tt_lib.tt_paged_attention(c, q.data_ptr(), 64, 32, ints([0, 1]).data_ptr(), None, 1, out.data_ptr(), 1, 2,
+                                           32, 0, 1.0, 0, 0, 1, ptr, size, torch.cuda.current_stream().cuda_stream)
+            assert rc == rc_want and bool(torch.all(out == 0)) == (rc_want != _lib.TT_OK)
 
 
 def test_cpu_tensors_are_refused():

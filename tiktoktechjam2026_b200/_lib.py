@@ -143,7 +143,10 @@ SIGNATURES = {
         [POINTER(KVCache), c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int,
          c_float, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p],
     ),
-    "tt_paged_attention_workspace_bytes": (c_int, [c_int, c_int, c_int, c_int, POINTER(c_size_t)]),
+    "tt_paged_attention_workspace_bytes": (
+        c_int,
+        [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, POINTER(c_size_t)],
+    ),
     "tt_model_create": (c_int, [POINTER(ModelDesc), POINTER(c_void_p)]),
     "tt_model_destroy": (None, [c_void_p]),
     "tt_workspace_alloc": (c_int, [c_size_t, POINTER(c_void_p)]),

@@ -125,9 +125,16 @@ int launch_paged_rows(PagedParams p, int row_lo, int row_hi, int sm_count, cudaS
   return launch_paged_join<T, HD, L::TK, kRowsMax, kRowsMax, 256>(p, kRowsMax / p.group, kRowsMinTiles, stream);
 }
 
-// Cache that one block of the kernel without cuts may have to stream: at more,
-// a lone long sequence would take longer on its block than cut over the GPU.
+// Whether a call takes the kernel without cuts (one block per sequence and KV
+// head): no sequence has more rows than fit an item, and none can have more
+// cache in sight than a block streams in some 10 us (a lone longer one would
+// take longer on its block than cut over the GPU).
 constexpr long long kItemBytes = 640 * 1024;
+bool paged_item_route(int stored_hd, long long max_rows, int window, int sinks, long long room) {
+  const long long reach = static_cast<long long>(window) + sinks + kRowsMax;  // keys that a window leaves an item
+  const long long keys = window > 0 && reach < room ? reach : room;
+  return max_rows <= kRowsMax && keys * stored_hd * 4 <= kItemBytes;
+}
 
 template <typename T, int HD>
 int launch_paged_item(const PagedParams& p, cudaStream_t stream) {
@@ -172,13 +179,8 @@ int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t str
 // Each sequence goes by its own number of query rows; max_rows only saves
 // launches whose kernel could have no work.
 template <typename T, int HD>
-int launch_paged(const PagedParams& p, int max_rows, int sm_count, cudaStream_t stream) {
-  if (max_rows <= kRowsMax) {
-    const long long room = static_cast<long long>(p.table_width) << p.page_shift;
-    const long long reach = static_cast<long long>(p.window) + p.sinks + kRowsMax;  // keys that a window leaves an item
-    const long long keys = p.window > 0 && reach < room ? reach : room;
-    if (p.batch > 0 && p.batch <= 65535 && keys * HD * 4 <= kItemBytes) return launch_paged_item<T, HD>(p, stream);
-  }
+int launch_paged(const PagedParams& p, bool items, int max_rows, int sm_count, cudaStream_t stream) {
+  if (items) return launch_paged_item<T, HD>(p, stream);
   if (max_rows <= kRowsMax) return launch_paged_rows<T, HD>(p, 0, 0x7fffffff, sm_count, stream);
   // With few (sequence, KV head) pairs the chunk kernel takes short sequences
   // along, at most two per SM: a second pair of launches that finds no short
@@ -190,13 +192,13 @@ int launch_paged(const PagedParams& p, int max_rows, int sm_count, cudaStream_t 
 }
 
 template <typename T>
-int launch_paged_t(const PagedParams& p, int hd, int max_rows, int sm_count, cudaStream_t stream) {
+int launch_paged_t(const PagedParams& p, int hd, bool items, int max_rows, int sm_count, cudaStream_t stream) {
   switch (hd) {
-    case 16: return launch_paged<T, 16>(p, max_rows, sm_count, stream);
-    case 32: return launch_paged<T, 32>(p, max_rows, sm_count, stream);
-    case 64: return launch_paged<T, 64>(p, max_rows, sm_count, stream);
-    case 128: return launch_paged<T, 128>(p, max_rows, sm_count, stream);
-    default: return launch_paged<T, 256>(p, max_rows, sm_count, stream);
+    case 16: return launch_paged<T, 16>(p, items, max_rows, sm_count, stream);
+    case 32: return launch_paged<T, 32>(p, items, max_rows, sm_count, stream);
+    case 64: return launch_paged<T, 64>(p, items, max_rows, sm_count, stream);
+    case 128: return launch_paged<T, 128>(p, items, max_rows, sm_count, stream);
+    default: return launch_paged<T, 256>(p, items, max_rows, sm_count, stream);
   }
 }
 
@@ -321,15 +323,19 @@ int tt_cache_copy_pages(const tt_kv_cache* cache, const int* src, const int* dst
   });
 }
 
-int tt_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int max_q_len, size_t* bytes) {
+int tt_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int max_q_len, int window, int sinks,
+                                       int table_width, int page, size_t* bytes) {
   return guarded([&]() -> int {
     DeviceState* ds;
     if (int rc = current_device_state(&ds)) return rc;
     if (!bytes) return fail(TT_ERR_ARG, "null argument");
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0)
       return fail(TT_ERR_SHAPE, "heads %d must be a multiple of kv_heads %d", heads, kv_heads);
-    (void)max_q_len;
-    return paged_workspace(head_dim, ds->sm_count, bytes);
+    if (int rc = paged_workspace(head_dim, ds->sm_count, bytes)) return rc;
+    if (max_q_len > 0 && paged_item_route(stored_head_dim(head_dim), static_cast<long long>(max_q_len) * (heads / kv_heads),
+                                          window, sinks, static_cast<long long>(table_width) * page))
+      *bytes = 0;
+    return TT_OK;
   });
 }
 
@@ -342,7 +348,7 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
     if (int rc = current_device_state(&ds)) return rc;
     CacheParams c;
     if (int rc = cache_params(cache, true, false, &c)) return rc;
-    if ((n_tokens > 0 && (!q || !out)) || !cu_q || !workspace) return fail(TT_ERR_ARG, "null argument");
+    if ((n_tokens > 0 && (!q || !out)) || !cu_q) return fail(TT_ERR_ARG, "null argument");
     if (n_tokens < 0 || batch < 0 || heads <= 0 || heads % c.kv_heads != 0 || heads / c.kv_heads > 128)
       return fail(TT_ERR_SHAPE, "invalid sizes (n_tokens %d, batch %d, heads %d, kv_heads %d)", n_tokens, batch, heads,
                   c.kv_heads);
@@ -352,12 +358,16 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
     if (stored_head_dim(head_dim) != cache->head_dim)
       return fail(TT_ERR_SHAPE, "head_dim %d is stored %d wide, the cache has %d", head_dim, stored_head_dim(head_dim),
                   cache->head_dim);
-    if (workspace_bytes < need)
-      return fail(TT_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || q_token_stride % 8 != 0 || q_head_stride % 8 != 0)
-      return fail(TT_ERR_ALIGN, "q, out and workspace must be 16-byte aligned, q's strides multiples of 8");
     const int group = heads / c.kv_heads;
     if (static_cast<long long>(n_tokens) * group >= 1LL << 30) return fail(TT_ERR_SHAPE, "too many query rows");
+    const int max_rows = (max_q_len > 0 && max_q_len < n_tokens ? max_q_len : n_tokens) * group;
+    const bool items = batch > 0 && batch <= 65535 &&
+                       paged_item_route(cache->head_dim, max_rows, window, sinks,
+                                        static_cast<long long>(c.table_width) << c.page_shift);
+    if (!items && (!workspace || workspace_bytes < need))
+      return fail(TT_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
+    if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || q_token_stride % 8 != 0 || q_head_stride % 8 != 0)
+      return fail(TT_ERR_ALIGN, "q, out and workspace must be 16-byte aligned, q's strides multiples of 8");
     if (n_tokens == 0) return TT_OK;
     PagedParams p;
     memset(&p, 0, sizeof(p));
@@ -391,10 +401,9 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
     p.scale_log2 = scale * 1.4426950408889634f;
     p.err = ds->err;
     p.timeout_ns = g_timeout_ns.load();
-    const int max_rows = (max_q_len > 0 && max_q_len < n_tokens ? max_q_len : n_tokens) * group;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return is_bf16 ? launch_paged_t<__nv_bfloat16>(p, cache->head_dim, max_rows, ds->sm_count, s)
-                   : launch_paged_t<__half>(p, cache->head_dim, max_rows, ds->sm_count, s);
+    return is_bf16 ? launch_paged_t<__nv_bfloat16>(p, cache->head_dim, items, max_rows, ds->sm_count, s)
+                   : launch_paged_t<__half>(p, cache->head_dim, items, max_rows, ds->sm_count, s);
   });
 }
 

@@ -5,23 +5,32 @@
 // One CTA per SM is one worker.  An item is two tiles ("halves") of up to 128
 // query rows each (one at head_dim 256); a row is (token, head of the KV
 // head's group), so grouped heads share every K and V tile.  Both halves read
-// the same ring of K and V tiles, which one producer warp fills: each page, or
-// the part of it inside the tile, is one TMA box per 64 features, and a page
-// that does not exist is fetched out of bounds, i.e. as zeros.  Each half has
-// 4 softmax warps (a whole row per thread) and its own MMA-issuing warp:
-//   S = Q K^T         TMEM, BN FP32 columns, NSB buffers per half
+// the same ring of K and V tiles (64 keys), which one producer warp fills: each
+// page, or the part of it inside the tile, is one TMA box per 64 features, and a
+// page that does not exist is fetched out of bounds, i.e. as zeros.  Each half
+// has 4 softmax warps (a whole row per thread) and two issuing warps:
+//   S = Q K^T         TMEM, 64 FP32 columns, NSB buffers
 //   P = 2^(S - m)     FP16/BF16 pairs written over the S it came from
 //   O += P V          P from TMEM, V as it lies in the page (MN-major operand)
-// The softmax is the bound below head_dim 128 (one exponential per score), so
-// part of the exponentials runs as a polynomial on the FMA pipe, the reference
-// maximum m moves only when a tile exceeds it by 2^8 (then O and l are
-// rescaled), and S runs up to NSB - 1 tiles ahead.  At head_dim 128 the tensor
-// core bounds it: key tiles of 128 keep the Q operand's shared-memory reads at
-// the rate of the MMA (64-wide ones read 1.5 times what the pipe can fetch),
-// and P.V of a tile's first 64 keys runs while the others' exponentials do.
-// A half skips the tiles that none of its rows sees.
-// The rows of V past a sequence's end in its last page may hold anything
-// (0 * NaN would reach the sum): a spare warp zeroes them in shared memory.
+// A quarter of the exponentials (3/8 up to head_dim 32) runs as a polynomial on
+// the FMA pipe, the reference maximum m moves only when a tile exceeds it by
+// 2^8 (then O and l are rescaled), and S runs up to NSB - 1 tiles ahead.  A half
+// skips the tiles that none of its rows sees.  V rows past a sequence's end in
+// its last page may hold anything (0 * NaN would reach the sum): the score
+// issuer of half 0 zeroes them in shared memory.
+//
+// What bounds it: a tile of 64 keys x 256 rows takes 1700-1850 cycles.  At
+// head_dim 128 the tensor core needs 1280 of them (Q K^T with N = 64 runs at 48
+// cycles per MMA, the rate of its operand reads from shared memory; P V at 64)
+// and is active 59 % of the time at the 1.54 GHz that the power limit leaves
+// (2048 new tokens over 30k keys, 16 heads over 4: 1.03 PFLOP/s).  Below that
+// the softmax warps bound it, two per scheduler and each a chain of TMEM read,
+// maximum, exponentials, TMEM write; the share of the polynomial does not
+// matter (0 to 3 of 8 measured alike).  Measured and left out: key tiles of 128
+// with P over S (one S buffer: the halves fall into step and wait for the
+// tensor core together, 4946 cycles per 128 keys) or beside it (582 us where
+// this takes 508); one issuing warp per half (550); more code than the
+// instruction cache holds (141 KB of it: 104 us for 32 prompts, 86 now).
 #pragma once
 
 #include <type_traits>
@@ -407,8 +416,8 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   } else if (warp >= L::W_S && warp < L::W_S + 2 * NT) {
     // -------------------------------------------------------------- issuers of a half
     // Scores and P.V are issued by warps of their own: an issuer's loop is a
-    // chain of waits and short bursts, and one warp doing both took longer per
-    // tile than the softmax.  A warp walks its loop as a whole on values that
+    // chain of waits (115 cycles even for a phase long complete) and short
+    // bursts.  A warp walks its loop as a whole on values that
     // shuffles make warp-uniform, and one elected lane issues: in a region of a
     // single lane every operand would go through vector registers.
     if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_OTHER));

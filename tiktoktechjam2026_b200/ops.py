@@ -241,9 +241,14 @@ def _cache(k: Optional[torch.Tensor], v: Optional[torch.Tensor], tables: torch.T
                    layers, pages, kv_heads, page, head_dim, slots, width)
 
 
+# The handle of the device's current stream: the call PyTorch itself launches with where it exists.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _run(device: int, fn, cache: KVCache, *args) -> None:
     """Calls a libtt_b200 entry point on the device's current stream."""
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = _raw_stream(device)
     if torch.cuda.current_device() == device:
         rc = fn(byref(cache), *args, stream)
     else:
@@ -354,11 +359,13 @@ def cache_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch
 _paged_ws_bytes: Dict[tuple, int] = {}
 
 
-def _paged_workspace_bytes(device: int, heads: int, kv_heads: int, head_dim: int) -> int:
+def _paged_workspace_bytes(key: tuple) -> int:
+    device, batch_small, rows, heads, kv_heads, *rest = key
     nbytes = c_size_t()
     with torch.cuda.device(device):
-        check(lib().tt_paged_attention_workspace_bytes(heads, kv_heads, head_dim, 0, nbytes))
-    _paged_ws_bytes[device, heads, kv_heads, head_dim] = int(nbytes.value)
+        check(lib().tt_paged_attention_workspace_bytes(
+            heads, kv_heads, rest[0], rows // (heads // kv_heads) if batch_small else 0, *rest[1:], nbytes))
+    _paged_ws_bytes[key] = int(nbytes.value)
     return int(nbytes.value)
 
 
@@ -395,11 +402,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out = torch.empty(n, heads * hd, dtype=dtype, device=q.device)
     elif (out.shape != (n, heads * hd) or out.dtype is not dtype or out.get_device() != dev or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous [{n}, {heads * hd}] tensor of q's dtype on cuda:{dev}")
-    need = _paged_ws_bytes.get((dev, heads, c.kv_heads, hd))
+    bound = n if max_q_len is None or not 0 < max_q_len < n else max_q_len
+    rows = bound * (heads // c.kv_heads)
+    # (More rows than an item holds: the workspace no longer depends on them.)
+    key = (dev, batch < 65536, rows if rows <= 16 else 1 << 20, heads, c.kv_heads, hd, window, sinks, c.table_width, c.page)
+    need = _paged_ws_bytes.get(key)
     if need is None:
-        need = _paged_workspace_bytes(dev, heads, c.kv_heads, hd)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        need = _paged_workspace_bytes(key)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _run(dev, lib().tt_paged_attention, c, q.data_ptr(), st[0], st[1], cu, sl, batch, out.data_ptr(), n, heads, hd,
-         dtype is torch.bfloat16, hd ** -0.5 if scale is None else scale, window, sinks,
-         n if max_q_len is None else max_q_len, ws.data_ptr(), need)
+         dtype is torch.bfloat16, hd ** -0.5 if scale is None else scale, window, sinks, bound,
+         ws.data_ptr() if need else None, need)
     return out
