@@ -228,6 +228,31 @@ def test_attention_one_long_sequence(tt_lib):
 
 
 @gpu
+@pytest.mark.parametrize("news_of", ["tokens", "mixed"])
+def test_attention_many_sequences(tt_lib, news_of):
+    """More sequences than a block has threads, in tables wide enough that items may be cut; some are empty."""
+    rng = random.Random(5)
+    n = 1300
+    news = [rng.choice([1, 1, 1, 0, 3]) if news_of == "tokens" or i % 9 else rng.randint(17, 40) for i in range(n)]
+    totals = [t + rng.choice([0, 1, 30, 64, rng.randint(0, 200)]) for t in news]
+    totals[7] = news[7] + 1900
+    book = Book(77, totals, 1, 128, 64, torch.float16, slots=1400)
+    check_attention(book, news, 2, torch.float16)
+
+
+@gpu
+def test_attention_no_sequence(tt_lib):
+    """No sequence at all, and sequences without tokens: every row is zero."""
+    book = Book(1, [20, 40], 2, 64, 16, torch.float16)
+    q = torch.randn(300, 4, 64, device=DEV).half()
+    for cu in ([0], [0, 0, 0], [300, 300, 300]):
+        for bound in (1, None):
+            got = ops.paged_attention(q, book.pages_k, book.pages_v, book.tables, book.lens, ints(cu), max_q_len=bound)
+            assert torch.all(got == 0)
+    assert ops.paged_attention(q[:0], book.pages_k, book.pages_v, book.tables, book.lens, ints([0, 0, 0])).shape == (0, 256)
+
+
+@gpu
 def test_attention_pool_past_2_31_bytes(tt_lib):
     """Pages past 2^31 values from the start of the pool, K and V interleaved in one buffer."""
     P, KH, page, hd = 36000, 2, 256, 64

@@ -361,7 +361,11 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
     const int group = heads / c.kv_heads;
     if (static_cast<long long>(n_tokens) * group >= 1LL << 30) return fail(TT_ERR_SHAPE, "too many query rows");
     const int max_rows = (max_q_len > 0 && max_q_len < n_tokens ? max_q_len : n_tokens) * group;
-    const bool items = batch > 0 && batch <= 65535 &&
+    if (batch == 0 && n_tokens > 0)  // no sequence has these rows
+      return check_cuda(cudaMemsetAsync(out, 0, static_cast<size_t>(n_tokens) * heads * head_dim * 2,
+                                        static_cast<cudaStream_t>(stream)),
+                        "cudaMemsetAsync");
+    const bool items = batch <= 65535 &&
                        paged_item_route(cache->head_dim, max_rows, window, sinks,
                                         static_cast<long long>(c.table_width) << c.page_shift);
     if (!items && (!workspace || workspace_bytes < need))

@@ -33,8 +33,6 @@
 // instruction cache holds (141 KB of it: 104 us for 32 prompts, 86 now).
 #pragma once
 
-#include <type_traits>
-
 #include "tt_attention.cuh"  // max3
 #include "tt_paged_attn.cuh"
 
