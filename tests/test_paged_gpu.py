@@ -228,6 +228,19 @@ def test_attention_one_long_sequence(tt_lib):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [16, 64, 128, 256])
+@pytest.mark.parametrize("seqs", [1, 2, 3])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (4000, 5)])
+def test_attention_few_long_sequences(tt_lib, dtype, hd, seqs, window, sinks):
+    """Short rows over long caches, few and more (sequence, KV head) pairs than a piece per SM is worth."""
+    past = [11003, 4097, 0][:seqs]
+    news = [1, 2, 3][:seqs]
+    book = Book(hd + seqs, [n + p for n, p in zip(news, past)], 8, hd, 32, dtype)
+    check_attention(book, news, 16, dtype, window=window, sinks=sinks)
+
+
+@gpu
 @pytest.mark.parametrize("news_of", ["tokens", "mixed"])
 def test_attention_many_sequences(tt_lib, news_of):
     """More sequences than a block has threads, in tables wide enough that items may be cut; some are empty."""

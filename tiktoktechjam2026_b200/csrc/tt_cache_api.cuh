@@ -70,8 +70,10 @@ int cache_params(const tt_kv_cache* c, bool values, bool counts, CacheParams* ou
 }
 
 // ---------------------------------------------------------------- attention
-// Sequences of at most this many query rows (tokens * group) take the kernel
-// for short chunks, whose items hold that many rows.
+// Sequences of at most this many query rows (tokens * group) take the kernels
+// for short chunks, whose items hold that many rows.  In us, those against the
+// chunk kernel: 16 rows, 16 sequences of 8000 keys, 8 KV heads of 128, 109 and
+// 118 (64 of 2000, heads of 64: 62 and 101); 32 rows 195 and 128 (109 and 103).
 constexpr int kRowsMax = 16;
 // Key tiles that a worker takes at least: shorter pieces would cost more in
 // joining than they save.
@@ -127,8 +129,10 @@ int launch_paged_rows(PagedParams p, int row_lo, int row_hi, int sm_count, cudaS
 
 // Whether a call takes the kernel without cuts (one block per sequence and KV
 // head): no sequence has more rows than fit an item, and none can have more
-// cache in sight than a block streams in some 10 us (a lone longer one would
-// take longer on its block than cut over the GPU).
+// cache in sight than a block streams in some 15 us.  In us, this against cut
+// pieces, 8 KV heads of 128: one sequence of 500 keys 13 and 20, of 8000 98 and
+// 52; 64 of 1000 54 and 62, 64 of 100 to 8000 217 and 193 (the last blocks run
+// alone).
 constexpr long long kItemBytes = 640 * 1024;
 bool paged_item_route(int stored_hd, long long max_rows, int window, int sinks, long long room) {
   const long long reach = static_cast<long long>(window) + sinks + kRowsMax;  // keys that a window leaves an item
@@ -181,11 +185,19 @@ int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t str
 template <typename T, int HD>
 int launch_paged(const PagedParams& p, bool items, int max_rows, int sm_count, cudaStream_t stream) {
   if (items) return launch_paged_item<T, HD>(p, stream);
-  if (max_rows <= kRowsMax) return launch_paged_rows<T, HD>(p, 0, 0x7fffffff, sm_count, stream);
+  const long long pairs = static_cast<long long>(p.batch) * p.kv_heads;
+  // With a handful of (sequence, KV head) pairs a piece for every warp would
+  // divide an item into a hundred parts; the chunk kernel has a piece per SM.
+  // One token over 8000 keys, 4 heads to each KV head of 128, in us, chunk
+  // kernel and this: 8 pairs 34 and 52, 16 pairs 38 and 44, 32 pairs 48 and 46.
+  constexpr int kFewPairs = 16;
+  if (max_rows <= kRowsMax && pairs > kFewPairs)
+    return launch_paged_rows<T, HD>(p, 0, 0x7fffffff, sm_count, stream);
   // With few (sequence, KV head) pairs the chunk kernel takes short sequences
-  // along, at most two per SM: a second pair of launches that finds no short
-  // sequence costs 8 us.
-  if (p.group > kRowsMax || static_cast<long long>(p.batch) * p.kv_heads <= 2ll * sm_count)
+  // along, at most two per SM: 8 sequences of 3000 keys, 8 KV heads of 128, 4 of them
+  // with 300 new tokens, 114 us against 132 with a second pair of launches, 32 such 177
+  // against 175, 64 such 263 against 241.
+  if (p.group > kRowsMax || pairs <= 2ll * sm_count)
     return launch_paged_chunk<T, HD>(p, 0, sm_count, stream);
   if (int rc = launch_paged_chunk<T, HD>(p, kRowsMax + 1, sm_count, stream)) return rc;
   return launch_paged_rows<T, HD>(p, 0, kRowsMax, sm_count, stream);

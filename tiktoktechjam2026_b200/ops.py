@@ -380,6 +380,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (``lens`` counts them).  With ``window`` a query sees the last ``window`` keys, itself included,
     and the first ``sinks`` ones.  A row that sees no key, or belongs to no sequence, is zero.
     ``head_dim`` 8 takes pages stored 16 wide; ``max_q_len``, if known, bounds every T.
+    What a page holds past its sequence's length is never used; an infinity or NaN among a sequence's
+    own keys and values may reach each of its rows, those whose mask hides it included.
     """
     c = _cache(k_pages, v_pages, tables, lens, None)
     dev = tables.get_device()
