@@ -1,0 +1,54 @@
+"""Paged-cache operators at the edges of what their arguments allow.
+
+Attention is held to the 64-bit formula and tolerance of ``test_paged_gpu``; everything else is compared exactly.
+"""
+
+import pytest
+import torch
+
+from test_paged_gpu import DEV, Book, check_attention, ints
+from tiktoktechjam2026_b200 import _lib, ops
+
+gpu = pytest.mark.gpu
+
+def word_is_clear():
+    word = _lib.c_uint()
+    return _lib.lib().tt_device_error(_lib.ctypes.byref(word), 0) == 0
+
+
+# ------------------------------------------------------------------------------------- order of kernels
+@gpu
+@pytest.mark.parametrize("news,past,hd,room", [
+    ([60, 33], [4, 0], 64, 0),            # chunk kernel, one key tile for each item: nothing is cut
+    ([300, 200], [5000, 0], 64, 0),       # chunk kernel, items are cut
+    ([1] * 40, [3] * 40, 128, 2000),      # rows kernel, one tile for each item, in a wide table
+    ([1] * 40, [1500] * 40, 128, 0),      # rows kernel, items are cut
+])
+def test_graph_node_after_attention_sees_its_rows(tt_lib, news, past, hd, room):
+    """A captured consumer of the output depends on the last kernel of the call alone: that one ends after the first."""
+    totals = [n + p for n, p in zip(news, past)]
+    book = Book(31, totals + ([room] if room else []), 2, hd, 64, torch.float16)
+    slots = book.slots[: len(news)].contiguous()
+    cu = [0]
+    for t in news:
+        cu.append(cu[-1] + t)
+    q = torch.randn(cu[-1], 4, hd, device=DEV).half()
+    out = torch.zeros(cu[-1], 4 * hd, dtype=torch.float16, device=DEV)
+    seen = torch.zeros_like(out)
+    call = lambda: ops.paged_attention(q, book.pages_k, book.pages_v, book.tables, book.lens, cu_q, slots=slots, out=out)  # noqa: E731
+    cu_q = ints(cu)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+        seen.copy_(out)
+    for _ in range(20):
+        q.normal_()
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = seen.clone()
+        call()
+        assert torch.equal(replayed, out)
+    assert word_is_clear()

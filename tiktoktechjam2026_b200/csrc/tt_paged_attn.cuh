@@ -369,9 +369,11 @@ __host__ __device__ constexpr long long paged_slot_floats() {
 //   O = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
 // One block per (worker, RB rows of the item).  A thread has four features of a
 // row; where rows are few, the parts are dealt over several threads and their
-// sums joined in a fixed order.  All blocks are resident at once, and most only
-// find that they have nothing to join: the schedule runs before the kernel
-// whose parts it reads has ended (programmatic launch).
+// sums joined in a fixed order.  The launch is programmatic, so blocks start on
+// SMs that the attention kernel has left and run the schedule beside its tail;
+// most find that they have nothing to join.  Those wait for the attention
+// kernel too: what comes after this grid (a node of a captured graph, say)
+// depends on this grid alone, so it must not end before that kernel has.
 
 struct JoinSum {
   float m, l;
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const PagedParams p
   long long per;
   const int c = blockIdx.x + 1;  // worker 0 starts at an item's beginning
   paged_schedule<TK, 1, THREADS>(p, tpi, min_tiles, c, &cut, &per);
-  if (cut.b < 0) return;
+  if (cut.b < 0) return pdl_wait();
   if (threadIdx.x < 32) {
     PagedWalk<TK> w;
     w.seek(p, cut, tpi);
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const PagedParams p
     }
   }
   __syncthreads();
-  if (n_after == 0) return;
+  if (n_after == 0) return pdl_wait();
   for (int k = threadIdx.x; k < n_after; k += THREADS)
     holds[k] = cur.tile_at(cur.at + k * per) < (k + 1 < n_after ? cur.tile_at(cur.at + (k + 1) * per) : cur.it.n);
   __syncthreads();
