@@ -52,3 +52,14 @@ def test_graph_node_after_attention_sees_its_rows(tt_lib, news, past, hd, room):
         call()
         assert torch.equal(replayed, out)
     assert word_is_clear()
+
+
+@gpu
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 3)])
+def test_attention_where_a_half_sees_few_tiles(tt_lib, hd, window, sinks):
+    """Of an item's two query tiles one is empty, or sees only some of the key tiles that pass through the ring."""
+    news, past = [20, 129, 200, 1], [9000, 3000, 64, 5000]
+    book = Book(hd, [n + p for n, p in zip(news, past)], 1, hd, 64, torch.bfloat16)
+    for heads in (1, 5):
+        check_attention(book, news, heads, torch.bfloat16, window=window, sinks=sinks)

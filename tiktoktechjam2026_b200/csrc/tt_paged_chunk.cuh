@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
   if (threadIdx.x == 64) {
     for (int i = 0; i < NST; ++i) {
       mbar_init(&bars[L::B_F + i], 1);
-      mbar_init(&bars[L::B_E + i], NT);
+      mbar_init(&bars[L::B_E + i], NT);  // per half: P.V of a tile it sees, the score issuer of another
       mbar_init(&bars[L::B_X + i], 1);
     }
     for (int i = 0; i < L::NSEG; ++i) {
@@ -418,6 +418,11 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
     // bursts.  A warp walks its loop as a whole on values that
     // shuffles make warp-uniform, and one elected lane issues: in a region of a
     // single lane every operand would go through vector registers.
+    // The score issuer waits for every stage in turn (it must not get a ring
+    // ahead: a parity tells two fills apart, not three), and each stage it waits
+    // for stays as it is until its half has handed it back: by P.V, which
+    // follows the scores, where the half sees the tile, and by the score issuer
+    // itself where it does not.  P.V then has nothing to wait for.
     if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_OTHER));
     const bool scores = warp < L::W_PV;
     const int h = __shfl_sync(~0u, warp - (scores ? L::W_S : L::W_PV), 0);
@@ -485,6 +490,8 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
               side = 0;
               side_ph ^= 1;
             }
+          } else if (lane == 0) {
+            mbar_arrive(&bars[L::B_E + st]);
           }
           if (++st == NST) {
             st = 0;
@@ -497,13 +504,13 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
 #pragma unroll 1
         for (; i < i1; ++i) {
           const bool on = i < a || (i >= c && i < e);
-          if (i == fix_at) {
-            if (!(ok = chunk_wait_warp(&bars[L::B_X + st], (fixed >> st) & 1, wd, 0x53b))) break;
-            fixed ^= 1u << st;
-          }
+          const bool fix = i == fix_at;
           if (on) {
             if (first) ok = chunk_wait_warp(&b[L::H_OR + side], side_ph ^ 1, wd, 0x539);
-            if (!(ok = ok && chunk_wait_warp(&b[L::H_PF + buf], buf_ph, wd, 0x538))) break;
+            ok = ok && chunk_wait_warp(&b[L::H_PF + buf], buf_ph, wd, 0x538);
+            // (After P: the stage then holds this tile, so the zeroing before this one is over and the parity exact.)
+            if (fix) ok = ok && chunk_wait_warp(&bars[L::B_X + st], (fixed >> st) & 1, wd, 0x53b);
+            if (!ok) break;
             tc_fence_after();
             const uint64_t dv = dv0 + (st * L::KV_BYTES >> 4);
             const uint32_t tO = tS + L::TMEM_O + side * HD, tP = tS + buf * BN;
@@ -525,14 +532,9 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
               side = 0;
               side_ph ^= 1;
             }
-          } else {  // not seen by this half: hand the stage back once it is there
-            if (!(ok = chunk_wait_warp(&bars[L::B_F + st], ph, wd, 0x53a))) break;
-            if (lane == 0) mbar_arrive(&bars[L::B_E + st]);
           }
-          if (++st == NST) {
-            st = 0;
-            ph ^= 1;
-          }
+          if (fix) fixed ^= 1u << st;
+          if (++st == NST) st = 0;
         }
       }
     }
