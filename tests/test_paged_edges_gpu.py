@@ -63,3 +63,21 @@ def test_attention_where_a_half_sees_few_tiles(tt_lib, hd, window, sinks):
     book = Book(hd, [n + p for n, p in zip(news, past)], 1, hd, 64, torch.bfloat16)
     for heads in (1, 5):
         check_attention(book, news, heads, torch.bfloat16, window=window, sinks=sinks)
+
+
+@gpu
+def test_compact_skips_entries_that_name_a_free_page(tt_lib):
+    """A table entry whose page has no count stays as it is; the live pages move as ever."""
+    k = torch.randn(2, 8, 1, 16, 16, device=DEV).half()
+    v = torch.randn(2, 8, 1, 16, 16, device=DEV).half()
+    k0, v0 = k.clone(), v.clone()
+    tables, lens, refs = ints([[2, 7, -1], [6, 5, 9]]), ints([32, 0]), ints([0, 0, 1, 0, 0, 0, 0, 1])
+    for _ in range(3):  # (the call's scratch is memory that earlier work has written)
+        junk = torch.full((64,), 1 << 28, dtype=torch.int32, device=DEV)
+        del junk
+        live = ops.cache_compact(k, v, tables, lens, refs)
+        assert live.item() == 2
+        assert tables.tolist() == [[0, 1, -1], [6, 5, 9]] and refs.tolist() == [1, 1, 0, 0, 0, 0, 0, 0]
+    for a, b in ((2, 0), (7, 1)):
+        k0[:, b], v0[:, b] = k0[:, a], v0[:, a]
+    assert torch.equal(k, k0) and torch.equal(v, v0)

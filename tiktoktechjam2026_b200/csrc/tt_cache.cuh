@@ -373,7 +373,8 @@ __global__ void __launch_bounds__(256)
 
 // Plan of compact, n = number of live pages: the k-th live page with index >=
 // n goes to the k-th free index below n.  scratch: [0] moves, [1] n, then
-// rank[n_pages] (k of a moving page), src[n_pages], dst[n_pages].
+// rank[n_pages] (k of a moving page, -1 for another one from n on), src[n_pages],
+// dst[n_pages].
 __global__ void __launch_bounds__(kCacheThreads) cache_compact_plan_kernel(const CacheParams c, int* scratch, int* live) {
   int mine = 0;
   for (int p = threadIdx.x; p < c.n_pages; p += kCacheThreads) mine += c.refs[p] > 0;
@@ -390,10 +391,8 @@ __global__ void __launch_bounds__(kCacheThreads) cache_compact_plan_kernel(const
     int total;
     const int both = block_scan((hole ? 1 : 0) + (move ? 1 << 16 : 0), &total);
     if (hole) dst[holes + (both & 0xffff)] = p;
-    if (move) {
-      rank[p] = moves + (both >> 16);
-      src[rank[p]] = p;
-    }
+    if (p >= n && p < c.n_pages) rank[p] = move ? moves + (both >> 16) : -1;
+    if (move) src[moves + (both >> 16)] = p;
     holes += total & 0xffff;
     moves += total >> 16;
   }
@@ -418,7 +417,9 @@ __global__ void __launch_bounds__(512) cache_compact_kernel(const CacheParams c,
     for (long long x = at; x < static_cast<long long>(c.n_slots) * c.table_width; x += step) {
       int* e = c.tables + x / c.table_width * c.table_stride + x % c.table_width;
       const int p = *e;
-      if (p >= n && p < c.n_pages) *e = dst[rank[p]];
+      if (p < n || p >= c.n_pages) continue;
+      const int k = rank[p];
+      if (k >= 0) *e = dst[k];  // an entry that names a free page stays
     }
   for (long long k = at; k < moves; k += step) {
     c.refs[dst[k]] = c.refs[src[k]];
