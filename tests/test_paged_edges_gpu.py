@@ -11,6 +11,22 @@ from tiktoktechjam2026_b200 import _lib, ops
 
 gpu = pytest.mark.gpu
 
+# Calls for each kernel of the attention: (new tokens, tokens before them, KV heads, query heads).  "item": short rows
+# over short tables; "rows": short rows, tables past 640 KB of cache, more than 16 (sequence, KV head) pairs; "chunk":
+# more than 16 rows; "few": short rows over a long cache, at most 16 pairs.
+LONG = {16: 11000, 32: 6000, 64: 3000, 128: 1500, 256: 800}
+
+
+def call_of(route, hd):
+    if route == "item":
+        return [1, 2, 3, 1], [0, 15, 297, 63], 2, 4
+    if route == "rows":
+        return [1, 2, 1, 4, 1, 1, 3, 1, 1], [LONG[hd], 5, 64, 700, 0, 129, LONG[hd] // 2, 1, 300], 2, 4
+    if route == "few":
+        return [1, 3], [LONG[hd], 70], 2, 4
+    return [1, 130, 40, 300], [300, 64, 500, 0], 2, 4
+
+
 def word_is_clear():
     word = _lib.c_uint()
     return _lib.lib().tt_device_error(_lib.ctypes.byref(word), 0) == 0
@@ -81,3 +97,26 @@ def test_compact_skips_entries_that_name_a_free_page(tt_lib):
     for a, b in ((2, 0), (7, 1)):
         k0[:, b], v0[:, b] = k0[:, a], v0[:, a]
     assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+# ---------------------------------------------------------------------------------------------- scale
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("route", ["item", "rows", "few", "chunk"])
+@pytest.mark.parametrize("scale", [-0.25, 0.0, -0.0, 0.5, 1e-30])
+def test_attention_scales(tt_lib, dtype, hd, route, scale):
+    """Any finite scale, on every kernel: hidden keys stay hidden whatever its sign."""
+    news, past, kv_heads, heads = call_of(route, hd)
+    book = Book(hd + 1, [n + p for n, p in zip(news, past)], kv_heads, hd, 64, dtype)
+    check_attention(book, news, heads, dtype, scale=scale)
+    check_attention(book, news, heads, dtype, scale=scale, window=40, sinks=3)
+
+
+@gpu
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39, 3e38])
+def test_attention_refuses_a_scale_that_is_not_finite(tt_lib, scale):
+    book = Book(1, [20, 40], 2, 32, 16, torch.float16)
+    q = torch.randn(2, 4, 32, device=DEV).half()
+    with pytest.raises(_lib.TTError, match="scale"):
+        ops.paged_attention(q, book.pages_k, book.pages_v, book.tables, book.lens, ints([0, 1, 2]), scale=scale)

@@ -2,6 +2,7 @@
 // Included once, at the end of tt_b200.cu, whose launch helpers it uses.
 #pragma once
 
+#include <cmath>
 #include <exception>
 
 #include "tt_cache.cuh"
@@ -161,6 +162,11 @@ int launch_paged_chunk(PagedParams p, int row_lo, int sm_count, cudaStream_t str
   p.row_hi = 0x7fffffff;
   p.n_workers = sm_count;
   p.item_len = kChunkItemTiles * L::BN;
+  // This kernel masks and compares raw scores, which a positive factor does not
+  // reorder: a negative scale's sign goes into Q K^T, and a scale of zero is
+  // one so small that 2^(s - m) is 1 in FP32 for every score below 2^76.
+  p.negate = p.scale_log2 < 0.f;
+  p.scale_log2 = fmaxf(fabsf(p.scale_log2), 0x1p-100f);
   const int half_tokens = 128 / p.group, page = 1 << p.page_shift;
   CUtensorMap tq, tk, tv;
   {
@@ -365,6 +371,8 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
       return fail(TT_ERR_SHAPE, "invalid sizes (n_tokens %d, batch %d, heads %d, kv_heads %d)", n_tokens, batch, heads,
                   c.kv_heads);
     if (window < 0 || sinks < 0) return fail(TT_ERR_ARG, "window and sinks must not be negative (%d, %d)", window, sinks);
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2)) return fail(TT_ERR_ARG, "scale %g is not finite or too large", scale);
     size_t need = 0;
     if (int rc = paged_workspace(head_dim, ds->sm_count, &need)) return rc;
     if (stored_head_dim(head_dim) != cache->head_dim)
@@ -414,7 +422,7 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
     p.window = window < room ? window : 0;
     p.sinks = sinks < room ? sinks : room;
     p.out_hd = head_dim;
-    p.scale_log2 = scale * 1.4426950408889634f;
+    p.scale_log2 = scale_log2;
     p.err = ds->err;
     p.timeout_ns = g_timeout_ns.load();
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -46,7 +46,8 @@ struct PagedParams {
   int row_lo, row_hi;          // this launch serves sequences of row_lo .. row_hi query rows (T * group)
   int n_workers;
   int item_len;                // extra length of an item on the line, in keys: its queries' loads and its output
-  float scale_log2;
+  float scale_log2;            // scale log2 e; in the chunk kernel its size, and `negate` its sign
+  int negate;
   unsigned int* err;
   unsigned long long timeout_ns;
 };

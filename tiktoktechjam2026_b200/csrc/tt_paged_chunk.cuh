@@ -9,7 +9,7 @@
 // page, or the part of it inside the tile, is one TMA box per 64 features, and a
 // page that does not exist is fetched out of bounds, i.e. as zeros.  Each half
 // has 4 softmax warps (a whole row per thread) and two issuing warps:
-//   S = Q K^T         TMEM, 64 FP32 columns, NSB buffers
+//   S = +-Q K^T       TMEM, 64 FP32 columns, NSB buffers (the scale's sign)
 //   P = 2^(S - m)     FP16/BF16 pairs written over the S it came from
 //   O += P V          P from TMEM, V as it lies in the page (MN-major operand)
 // A quarter of the exponentials (3/8 up to head_dim 32) runs as a polynomial on
@@ -99,7 +99,9 @@ __device__ __forceinline__ uint64_t umma_sdesc_mn(uint32_t saddr, uint32_t lbo, 
 }
 
 // Instruction descriptor of kind::f16 with an FP32 accumulator: BF16 operands
-// set the A and B formats (bits 7 and 10), an MN-major B sets bit 16.
+// set the A and B formats (bits 7 and 10), an MN-major B sets bit 16.  Bit 13
+// negates A.
+constexpr uint32_t kIdescNegateA = 1u << 13;
 __host__ __device__ constexpr uint32_t umma_idesc_16(int M, int N, bool bf16, bool b_mn) {
   return umma_idesc_f16_f32(M, N) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
 }
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
       if (i1 < 0) break;
       bool first = true;
       if (scores) {
-        constexpr uint32_t idesc = umma_idesc_16(128, BN, PT::kBf16, false);
+        const uint32_t idesc = umma_idesc_16(128, BN, PT::kBf16, false) | (p.negate ? kIdescNegateA : 0u);
         const uint64_t dq0 = umma_sdesc(sbase + L::OFF_Q + h * NQ * L::Q_BYTES, kSbo, kSw);
         const uint64_t dk0 = umma_sdesc(sbase + L::OFF_K, kSbo, kSw);
 #pragma unroll 1

@@ -377,8 +377,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     q [tokens, heads, hs] (dense features, any token and head strides of whole 16 bytes); heads a
     multiple of the pages' kv_heads.  The T new tokens of a sequence are its last T positions
-    (``lens`` counts them).  With ``window`` a query sees the last ``window`` keys, itself included,
-    and the first ``sinks`` ones.  A row that sees no key, or belongs to no sequence, is zero.
+    (``lens`` counts them).  ``scale`` (hd ** -0.5 by default) is any finite number.  With ``window``
+    a query sees the last ``window`` keys, itself included, and the first ``sinks`` ones.  A row that
+    sees no key, or belongs to no sequence, is zero.
     ``head_dim`` 8 takes pages stored 16 wide; ``max_q_len``, if known, bounds every T.
     What a page holds past its sequence's length is never used; an infinity or NaN among a sequence's
     own keys and values may reach each of its rows, those whose mask hides it included.
