@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_paged_gpu import DEV, Book, check_attention, ints
-from tiktoktechjam2026_b200 import _lib, ops
+from tiktoktechjam2026_b200 import PagedKVCache, _lib, ops
 
 gpu = pytest.mark.gpu
 
@@ -120,3 +120,59 @@ def test_attention_refuses_a_scale_that_is_not_finite(tt_lib, scale):
     q = torch.randn(2, 4, 32, device=DEV).half()
     with pytest.raises(_lib.TTError, match="scale"):
         ops.paged_attention(q, book.pages_k, book.pages_v, book.tables, book.lens, ints([0, 1, 2]), scale=scale)
+
+
+# --------------------------------------------------------------------------------- reservations and their appends
+def _cache_with_one_sequence():
+    cache = PagedKVCache(1, 4, 1, 16, slots=4, max_len=96, page=16, device=DEV)
+    cache.k.zero_(), cache.v.zero_()
+    cu, slot = ints([0, 40]), ints([0])
+    status = cache.reserve(cu, slot)
+    cache.append(0, torch.ones(40, 1, 16, device=DEV).half(), torch.ones(40, 1, 16, device=DEV).half(), cu, slot,
+                 status=status)
+    cache.check()
+    return cache
+
+
+@gpu
+@pytest.mark.parametrize("between", ["reserve", "fork", "nothing"])
+def test_append_of_a_refused_reservation_writes_nothing(tt_lib, between):
+    """Whatever is reserved or forked after it: an append goes by the answer to its own reservation."""
+    cache = _cache_with_one_sequence()
+    k, v = cache.k.clone(), cache.v.clone()
+    cu, slots = ints([0, 24, 40]), ints([0, 1])
+    refused = cache.reserve(cu, slots)  # two pages, one is free
+    if between == "reserve":
+        cache.reserve(ints([0, 5]), ints([2]))
+        cache.check()
+    elif between == "fork":
+        cache.fork(ints([0]), ints([3]))
+        cache.check()
+        k, v = cache.k.clone(), cache.v.clone()  # (the child's copy of the partial page)
+    new = torch.full((40, 1, 16), 7.0, device=DEV).half()
+    cache.append(0, new, new, cu, slots, status=refused)
+    assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
+    with pytest.raises(RuntimeError, match="short"):
+        cache.check(refused)
+
+
+@gpu
+def test_append_of_an_accepted_reservation_survives_a_refused_call(tt_lib):
+    cache = _cache_with_one_sequence()
+    cu, slot = ints([0, 8]), ints([0])
+    granted = cache.reserve(cu, slot)
+    cache.fork(ints([0]), ints([0]))  # not empty
+    with pytest.raises(RuntimeError, match="empty"):
+        cache.check()
+    new = torch.full((8, 1, 16), 7.0, device=DEV).half()
+    cache.append(0, new, new, cu, slot, status=granted)
+    page = int(cache.tables[0, 2])
+    assert torch.all(cache.k[0, page, 0, 8:] == 7) and torch.all(cache.k[0, page, 0, :8] == 1)
+
+
+@gpu
+def test_append_names_its_reservation(tt_lib):
+    cache = _cache_with_one_sequence()
+    new = torch.zeros(8, 1, 16, device=DEV).half()
+    with pytest.raises(TypeError, match="status"):
+        cache.append(0, new, new, ints([0, 8]), ints([0]))

@@ -57,9 +57,10 @@ class PagedKVCache:
     def device(self) -> torch.device:
         return self.k.device
 
-    def check(self) -> None:
-        """Waits for the last ``reserve`` or ``fork`` and raises if it was refused (it then changed nothing)."""
-        status = int(self.status.item())
+    def check(self, status: Optional[torch.Tensor] = None) -> None:
+        """Waits for the ``reserve`` or ``fork`` that returned ``status`` (the last one without it) and raises if it
+        was refused (it then changed nothing)."""
+        status = int((self.status if status is None else status).item())
         if status > 0:
             raise RuntimeError(f"the page pool is {status} page(s) short")
         if status < 0:
@@ -68,14 +69,18 @@ class PagedKVCache:
                                 -3: "a child slot that is not empty or occurs twice"}[status])
 
     def reserve(self, cu_q: torch.Tensor, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Pages for the new tokens cu_q describes, which ``lens`` counts from then on; see ``ops.cache_reserve``."""
+        """Pages for the new tokens cu_q describes, which ``lens`` counts from then on; see ``ops.cache_reserve``.
+
+        Returns the reservation's status, which every ``append`` of these tokens takes.
+        """
         self.status = ops.cache_reserve(self.tables, self.lens, self.refs, cu_q, self.page, slots)
         return self.status
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
-               slots: Optional[torch.Tensor] = None) -> None:
-        """Writes one layer's K and V of the tokens just reserved (nothing if that was refused)."""
-        ops.cache_append(k, v, self.k[layer], self.v[layer], self.tables, self.lens, cu_q, slots, status=self.status)
+               slots: Optional[torch.Tensor] = None, *, status: torch.Tensor) -> None:
+        """Writes one layer's K and V of the tokens whose ``reserve`` returned ``status`` (nothing if it was refused:
+        the lengths do not count them, and the positions they would take hold other tokens)."""
+        ops.cache_append(k, v, self.k[layer], self.v[layer], self.tables, self.lens, cu_q, slots, status=status)
 
     def attend(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor, slots: Optional[torch.Tensor] = None, *,
                scale: Optional[float] = None, window: int = 0, sinks: int = 0,

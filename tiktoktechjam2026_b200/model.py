@@ -529,7 +529,7 @@ class B200Transformer(nn.Module):
                 cu_q = torch.zeros(batch + 1, dtype=torch.int32, device=x.device)
         rows = x.reshape(-1, cfg.d_model).contiguous()
         n = rows.shape[0]
-        cache.reserve(cu_q, slots)
+        status = cache.reserve(cu_q, slots)
         if check:
             cache.check()
         if n == 0:
@@ -544,7 +544,7 @@ class B200Transformer(nn.Module):
 
             q, k, vt = ops.qkv_projection(norm.view(1, n, -1), att.qkv_proj.weight, bias("attention.qkv_proj", att.qkv_proj),
                                           cfg.num_heads)
-            cache.append(i, k[0].transpose(0, 1), vt[0, :, :, :n].permute(2, 0, 1), cu_q, slots)
+            cache.append(i, k[0].transpose(0, 1), vt[0, :, :, :n].permute(2, 0, 1), cu_q, slots, status=status)
             ctx = cache.attend(i, q[0].transpose(0, 1), cu_q, slots, scale=att.scale, window=window, sinks=sinks,
                                max_q_len=max_q_len)
             rows, norm = ops.linear_residual_layernorm(ctx, att.out_proj.weight, bias("attention.out_proj", att.out_proj), rows,
