@@ -931,6 +931,10 @@ int tt_layernorm_rows(const float* x, const float* gamma, const float* beta, voi
   if (int rc = current_device_state(&ds)) return rc;
   if (!x || !gamma || !beta || !out || n_rows < 0) return fail(TT_ERR_ARG, "null argument");
   if (int rc = check_ln_width(d)) return rc;
+  // Widths of whole 128 are read and written in 16-byte pieces.
+  if (d % 128 == 0 && (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(gamma) |
+                       reinterpret_cast<uintptr_t>(beta) | reinterpret_cast<uintptr_t>(out)) % 16 != 0)
+    return fail(TT_ERR_ALIGN, "x, gamma, beta and out must be 16-byte aligned at width %d", d);
   return run_layernorm(x, gamma, beta, out, n_rows, d, eps, out_is_f16,
                        static_cast<cudaStream_t>(stream));
 }

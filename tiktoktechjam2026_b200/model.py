@@ -14,6 +14,7 @@ from __future__ import annotations
 import copy
 import ctypes
 import itertools
+import operator
 import weakref
 from dataclasses import dataclass
 from typing import Dict, Optional, Sequence
@@ -486,6 +487,31 @@ class B200Transformer(nn.Module):
         return out
 
 
+    def _layer_tensors(self, device: torch.device) -> list:
+        """Each layer's weights, FP32 biases and LayerNorm parameters in the order of ``extend``'s operators.
+
+        Raises unless all are on ``device``, the projections are FP16 and the shape has kernels.
+        """
+        cfg = self.config
+        _lib.check(_lib.lib().tt_route_describe(cfg.d_model, cfg.num_heads, 1, cfg.ffn_dim, None, 0))
+        index, kept = device.index, self._bias_fp32.get
+        norms = [layer.norm1 for layer in self.layers][1:] + [self.final_norm]
+        out = []
+        for i, (layer, nxt) in enumerate(zip(self.layers, norms)):
+            att, norm2 = layer.attention, layer.norm2
+            row = []
+            for name, linear in (("attention.qkv_proj", att.qkv_proj), ("attention.out_proj", att.out_proj),
+                                 ("ffn_in", layer.ffn_in), ("ffn_out", layer.ffn_out)):
+                weight = linear.weight
+                if weight.dtype is not torch.float16:
+                    raise RuntimeError("projection weights must be FP16: call convert_projections_to_fp16()")
+                row += weight, kept(f"layers.{i}.{name}", linear.bias)
+            row += norm2.weight, norm2.bias, nxt.weight, nxt.bias
+            if any(t.get_device() != index for t in row):
+                raise ValueError(f"layer {i} has parameters that are not on {device}")
+            out.append((att.scale, *row))
+        return out
+
     def extend(
         self,
         x: torch.Tensor,
@@ -521,6 +547,12 @@ class B200Transformer(nn.Module):
         if cache.k.shape[0] != cfg.num_layers or cache.k.shape[2] != cfg.num_heads or (
                 cache.head_dim != cfg.d_model // cfg.num_heads) or cache.k.dtype != torch.float16:
             raise ValueError("the cache does not have this model's layers, heads and FP16 pages")
+        window, sinks, max_q_len = operator.index(window), operator.index(sinks), max_q_len and operator.index(max_q_len)
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must not be negative")
+        layers, norm0 = self._layer_tensors(x.device), self.layers[0].norm1
+        if norm0.weight.get_device() != x.device.index or norm0.bias.get_device() != x.device.index:
+            raise ValueError(f"parameter on {norm0.weight.device}, tokens on {x.device}")
         if cu_q is None:
             batch, steps = x.shape[:2]
             max_q_len = steps
@@ -528,36 +560,30 @@ class B200Transformer(nn.Module):
             if steps == 0:
                 cu_q = torch.zeros(batch + 1, dtype=torch.int32, device=x.device)
         rows = x.reshape(-1, cfg.d_model).contiguous()
+        if rows.data_ptr() % 16:
+            rows = rows.clone()
         n = rows.shape[0]
+        eps, last = float(norm0.eps), cfg.num_layers - 1
+        if n:  # (first: it refuses a width without a kernel)
+            norm = ops.layernorm_rows(rows, norm0.weight, norm0.bias, eps)
         status = cache.reserve(cu_q, slots)
         if check:
             cache.check()
         if n == 0:
             return torch.empty_like(x)
-        eps, last = float(self.layers[0].norm1.eps), cfg.num_layers - 1
-        norm = ops.layernorm_rows(rows, self.layers[0].norm1.weight, self.layers[0].norm1.bias, eps)
-        for i, layer in enumerate(self.layers):
-            att, nxt = layer.attention, self.final_norm if i == last else self.layers[i + 1].norm1
-
-            def bias(name: str, linear: nn.Linear) -> torch.Tensor:
-                return self._bias_fp32.get(f"layers.{i}.{name}", linear.bias)
-
-            q, k, vt = ops.qkv_projection(norm.view(1, n, -1), att.qkv_proj.weight, bias("attention.qkv_proj", att.qkv_proj),
-                                          cfg.num_heads)
+        fused = cfg.d_model in (32, 64, 128, 256) and cfg.ffn_dim % 128 == 0
+        for i, (scale, w_qkv, b_qkv, w_out, b_out, w_in, b_in, w_ffn, b_ffn, ln_w, ln_b, next_w, next_b) in enumerate(layers):
+            q, k, vt = ops.qkv_projection(norm.view(1, n, -1), w_qkv, b_qkv, cfg.num_heads)
             cache.append(i, k[0].transpose(0, 1), vt[0, :, :, :n].permute(2, 0, 1), cu_q, slots, status=status)
-            ctx = cache.attend(i, q[0].transpose(0, 1), cu_q, slots, scale=att.scale, window=window, sinks=sinks,
+            ctx = cache.attend(i, q[0].transpose(0, 1), cu_q, slots, scale=scale, window=window, sinks=sinks,
                                max_q_len=max_q_len)
-            rows, norm = ops.linear_residual_layernorm(ctx, att.out_proj.weight, bias("attention.out_proj", att.out_proj), rows,
-                                                       layer.norm2.weight, layer.norm2.bias, eps)
+            rows, norm = ops.linear_residual_layernorm(ctx, w_out, b_out, rows, ln_w, ln_b, eps)
             out_type = torch.float32 if i == last else torch.float16
-            b_in, b_out = bias("ffn_in", layer.ffn_in), bias("ffn_out", layer.ffn_out)
-            if cfg.d_model in (32, 64, 128, 256) and cfg.ffn_dim % 128 == 0:
-                rows, norm = ops.ffn_residual_layernorm(norm, layer.ffn_in.weight, b_in, layer.ffn_out.weight, b_out, rows,
-                                                        nxt.weight, nxt.bias, eps, out_type)
+            if fused:
+                rows, norm = ops.ffn_residual_layernorm(norm, w_in, b_in, w_ffn, b_ffn, rows, next_w, next_b, eps, out_type)
             else:
-                hidden = ops.linear_gelu(norm, layer.ffn_in.weight, b_in)
-                rows, norm = ops.linear_residual_layernorm(hidden, layer.ffn_out.weight, b_out, rows, nxt.weight, nxt.bias,
-                                                           eps, out_type)
+                hidden = ops.linear_gelu(norm, w_in, b_in)
+                rows, norm = ops.linear_residual_layernorm(hidden, w_ffn, b_ffn, rows, next_w, next_b, eps, out_type)
         return norm.view(x.shape)
 
     def capture_graph(self, x: torch.Tensor, valid_token_mask: Optional[torch.Tensor] = None) -> "GraphedForward":
