@@ -176,3 +176,34 @@ def test_append_names_its_reservation(tt_lib):
     new = torch.zeros(8, 1, 16, device=DEV).half()
     with pytest.raises(TypeError, match="status"):
         cache.append(0, new, new, ints([0, 8]), ints([0]))
+
+
+# -------------------------------------------------------------------------------------- windows past 32 bits
+@gpu
+@pytest.mark.parametrize("route", ["item", "chunk"])
+def test_attention_window_of_any_size(tt_lib, route):
+    """A window or first tokens past every position are as good as all keys, also past 32 bits."""
+    news, past, kv_heads, heads = call_of(route, 64)
+    book = Book(3, [n + p for n, p in zip(news, past)], kv_heads, 64, 16, torch.float16)
+    q = torch.randn(sum(news), heads, 64, device=DEV).half()
+    cu = [0]
+    for t in news:
+        cu.append(cu[-1] + t)
+    call = lambda **kw: ops.paged_attention(q, book.pages_k, book.pages_v, book.tables, book.lens, ints(cu),  # noqa: E731
+                                            slots=book.slots, **kw)
+    want = call()
+    for window in (1 << 30, 2**31 - 1, 2**31, 2**32, 2**32 + 5, 2**40):
+        assert torch.equal(call(window=window), want)
+    for sinks in (2**31 - 1, 2**31, 2**32, 2**32 + 1):
+        torch.testing.assert_close(call(window=20, sinks=sinks), want, rtol=2e-3, atol=2e-3)
+
+
+@gpu
+def test_trim_behind_a_window_of_any_size(tt_lib):
+    tables, lens, refs = ints([[1, 0, 2, -1]]), ints([48]), ints([1, 1, 1])
+    for window, sinks in ((2**31, 0), (2**32, 0), (2**32 + 1, 0), (1, 2**32), (1, 2**31)):
+        ops.cache_release(tables, lens, refs, 16, window=window, sinks=sinks)
+        assert tables.tolist() == [[1, 0, 2, -1]] and lens.tolist() == [48] and refs.tolist() == [1, 1, 1]
+    with pytest.raises(_lib.TTError, match="negative"):
+        ops.cache_release(tables, lens, refs, 16, window=-(2**32))
+    assert lens.tolist() == [48]

@@ -258,6 +258,11 @@ def _run(device: int, fn, cache: KVCache, *args) -> None:
         check(rc)
 
 
+def _reach(tokens: int) -> int:
+    """A window or a number of first tokens for the 32-bit entry points: no position reaches 2^30."""
+    return max(-1, min(int(tokens), 1 << 30))
+
+
 def _batch(cu_q: torch.Tensor, slots: Optional[torch.Tensor], tables: torch.Tensor) -> Tuple[int, int, int]:
     """(address of cu_q, address of slots, sequences of the call)."""
     n, dev = cu_q.shape[0] - 1, tables.get_device()
@@ -316,7 +321,7 @@ def cache_release(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, 
     c = _cache(None, None, tables, lens, refs, page)
     n = tables.shape[0] if slots is None else slots.shape[0]
     dev = tables.get_device()
-    _run(dev, lib().tt_cache_release, c, _index(slots, "slots", dev), n, int(window), int(sinks))
+    _run(dev, lib().tt_cache_release, c, _index(slots, "slots", dev), n, _reach(window), _reach(sinks))
 
 
 def cache_fork(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
@@ -399,6 +404,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"{heads} query heads are not a multiple of {c.kv_heads} KV heads")
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
+    window, sinks = _reach(window), _reach(sinks)
     hd = hs if head_dim is None else int(head_dim)
     cu, sl, batch = _batch(cu_q, slots, tables)
     if out is None:
