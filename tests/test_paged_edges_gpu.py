@@ -207,3 +207,28 @@ def test_trim_behind_a_window_of_any_size(tt_lib):
     with pytest.raises(_lib.TTError, match="negative"):
         ops.cache_release(tables, lens, refs, 16, window=-(2**32))
     assert lens.tolist() == [48]
+
+
+# ------------------------------------------------------------------------------------------- hidden keys
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("heads", [1, 4])
+def test_hidden_values_weigh_nothing(tt_lib, dtype, hd, heads):
+    """The largest finite values at positions that a row does not see leave the row as it is, bit for bit."""
+    big = torch.finfo(dtype).max
+    book = Book(hd, [228], 1, hd, 32, dtype)
+    q = torch.randn(200, heads, hd, device=DEV).to(dtype)
+    row = book.tables[book.slot_of[0]].tolist()
+
+    def call(value, lo, hi, window):
+        v = book.pages_v.clone()
+        for u in range(lo, hi):
+            v[row[u // 32], :, u % 32] = value
+        return ops.paged_attention(q, book.pages_k, v, book.tables, book.lens, ints([0, 200]), slots=book.slots,
+                                   window=window)
+
+    late, none = call(big, 100, 228, 0), call(0.0, 100, 228, 0)
+    assert torch.equal(late[:72], none[:72])  # positions 28 .. 99
+    late, none = call(big, 0, 60, 30), call(0.0, 0, 60, 30)
+    assert torch.equal(late[62:], none[62:])  # positions 90 .. 227 see 61 and later

@@ -12,12 +12,12 @@
 //   S = +-Q K^T       TMEM, 64 FP32 columns, NSB buffers (the scale's sign)
 //   P = 2^(S - m)     FP16/BF16 pairs written over the S it came from
 //   O += P V          P from TMEM, V as it lies in the page (MN-major operand)
-// A quarter of the exponentials (3/8 up to head_dim 32) runs as a polynomial on
-// the FMA pipe, the reference maximum m moves only when a tile exceeds it by
-// 2^8 (then O and l are rescaled), and S runs up to NSB - 1 tiles ahead.  A half
-// skips the tiles that none of its rows sees.  V rows past a sequence's end in
-// its last page may hold anything (0 * NaN would reach the sum): the score
-// issuer of half 0 zeroes them in shared memory.
+// In FP16 a quarter of the exponentials (3/8 up to head_dim 32) runs as a
+// polynomial on the FMA pipe.  The reference maximum m moves only when a tile
+// exceeds it by 2^8 (then O and l are rescaled), and S runs up to NSB - 1 tiles
+// ahead.  A half skips the tiles that none of its rows sees.  V rows past a
+// sequence's end in its last page may hold anything (0 * NaN would reach the
+// sum): the score issuer of half 0 zeroes them in shared memory.
 //
 // What bounds it: a tile of 64 keys x 256 rows takes 1700-1850 cycles.  At
 // head_dim 128 the tensor core needs 1280 of them (Q K^T with N = 64 runs at 48
@@ -107,8 +107,8 @@ __host__ __device__ constexpr uint32_t umma_idesc_16(int M, int N, bool bf16, bo
 }
 
 // 2^x of a pair on the FMA pipe for any x: exp2_pair_fma_y (tt_ptx.cuh) with a
-// wider clamp, y = saturate((x + 126) / 256), because BF16 and the FP32 row
-// sum keep what FP16 rounds to zero.  The rounding of y costs 2^-17 in x.
+// wider clamp, y = saturate((x + 126) / 256), because the FP32 row sum keeps
+// what FP16 rounds to zero.  The rounding of y costs 2^-17 in x.
 constexpr float kExpYScale = 1.0f / 256.0f;
 constexpr float kExpYBias = 126.0f / 256.0f;
 __device__ __forceinline__ uint64_t exp2_pair_wide(uint64_t yy) {
@@ -230,9 +230,14 @@ __device__ __forceinline__ bool chunk_wait_warp(uint64_t* bar, uint32_t parity, 
   return __all_sync(0xffffffffu, chunk_wait(bar, parity, wd, site));
 }
 
-// Exponentials per 8 pairs on the FMA pipe.
-template <int HD>
-constexpr int kChunkExpFma = HD <= 32 ? 3 : 2;
+// Exponentials per 8 pairs on the FMA pipe.  None in BF16: the polynomial ends
+// at 2^-126 where MUFU gives 0, which FP16 rounds away and BF16 keeps, so that a
+// hidden key's value near the type's largest would count.  That costs 320 us
+// to 334 at head_dim 256 (2048 new tokens over 15k, 8 heads over 2), 425 to 437
+// at 32 (over 30k, 16 over 4) and nothing at 64 and 128; clearing hidden weights
+// or taking 2^-126 off again costs as much or more (128: 488 to 502-525).
+template <typename T, int HD>
+constexpr int kChunkExpFma = Pair16<T>::kBf16 ? 0 : HD <= 32 ? 3 : 2;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
@@ -724,8 +729,9 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
         const float y_scale = sl2 * kExpYScale, y_bias = fmaf(-m_use, kExpYScale, kExpYBias);
         uint64_t sum[2] = {f2_pack(l_run, 0.f), 0ull};
         // A hidden score gives 0 on MUFU and 2^-126 where the polynomial's
-        // clamp ends: nothing beside the row's largest term, which is at least
-        // 1, and a row that saw no key is known by its tiny sum.
+        // clamp ends: in the sum nothing beside the row's largest term, which is
+        // at least 1 (a row that saw no key is known by its tiny sum), and as a
+        // weight 0 in FP16.
 #pragma unroll
         for (int g = 0; g < BN / 32; ++g) {
           uint32_t pk[16];
@@ -733,7 +739,7 @@ __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
           for (int e = 0; e < 16; ++e) {
             uint64_t pp;
             const float s0 = __uint_as_float(sc[g][2 * e]), s1 = __uint_as_float(sc[g][2 * e + 1]);
-            if ((e & 7) < kChunkExpFma<HD>) {
+            if ((e & 7) < kChunkExpFma<T, HD>) {
               pp = exp2_pair_wide(f2_pack(fma_sat(s0, y_scale, y_bias), fma_sat(s1, y_scale, y_bias)));
             } else {
               const uint64_t xx = ffma2(f2_pack(s0, s1), sl2x2, negm);
