@@ -12,10 +12,9 @@
 //   S = +-Q K^T       TMEM, 64 FP32 columns, NSB buffers (the scale's sign)
 //   P = 2^(S - m)     FP16/BF16 pairs written over the S it came from
 //   O += P V          P from TMEM, V as it lies in the page (MN-major operand)
-// In FP16 a quarter of the exponentials (3/8 up to head_dim 32) runs as a
-// polynomial on the FMA pipe.  The reference maximum m moves only when a tile
-// exceeds it by 2^8 (then O and l are rescaled), and S runs up to NSB - 1 tiles
-// ahead.  A half skips the tiles that none of its rows sees.  V rows past a
+// In FP16 from head_dim 128 a quarter of the exponentials runs as a polynomial
+// on the FMA pipe.  The reference maximum m moves only when a tile exceeds it by
+// 2^8 (then O and l are rescaled), and S runs up to NSB - 1 tiles ahead.  A half skips the tiles that none of its rows sees.  V rows past a
 // sequence's end in its last page may hold anything (0 * NaN would reach the
 // sum): the score issuer of half 0 zeroes them in shared memory.
 //
@@ -25,8 +24,7 @@
 // and is active 59 % of the time at the 1.54 GHz that the power limit leaves
 // (2048 new tokens over 30k keys, 16 heads over 4: 1.03 PFLOP/s).  Below that
 // the softmax warps bound it, two per scheduler and each a chain of TMEM read,
-// maximum, exponentials, TMEM write; the share of the polynomial does not
-// matter (0 to 3 of 8 measured alike).  Measured and left out: key tiles of 128
+// maximum, exponentials, TMEM write.  Measured and left out: key tiles of 128
 // with P over S (one S buffer: the halves fall into step and wait for the
 // tensor core together, 4946 cycles per 128 keys) or beside it (582 us where
 // this takes 508); one issuing warp per half (550); more code than the
@@ -230,14 +228,18 @@ __device__ __forceinline__ bool chunk_wait_warp(uint64_t* bar, uint32_t parity, 
   return __all_sync(0xffffffffu, chunk_wait(bar, parity, wd, site));
 }
 
-// Exponentials per 8 pairs on the FMA pipe.  None in BF16: the polynomial ends
-// at 2^-126 where MUFU gives 0, which FP16 rounds away and BF16 keeps, so that a
-// hidden key's value near the type's largest would count.  That costs 320 us
-// to 334 at head_dim 256 (2048 new tokens over 15k, 8 heads over 2), 425 to 437
-// at 32 (over 30k, 16 over 4) and nothing at 64 and 128; clearing hidden weights
-// or taking 2^-126 off again costs as much or more (128: 488 to 502-525).
+// Exponentials per 8 pairs on the FMA pipe: two in FP16 from head_dim 128, where
+// they gain (us with them and without: 2048 new tokens over 15k keys, 8 heads
+// over 2 of 256, 320 and 334; over 30k, 16 over 4 of 128, 479 and 485; ragged
+// chunks, 32 over 8 of 128, 253 and 256).  None below: 16 over 4 of 64 469 and
+// 464, of 32 429 and 438, but 32 prompts of 1024, 8 heads of 32, 93 and 90 and of
+// 64 95 and 95, and the polynomial's error is the larger.  None in BF16: the
+// polynomial ends at 2^-126 where MUFU gives 0, which FP16 rounds away and BF16
+// keeps, so that a hidden key's value near the type's largest would count (256:
+// 320 and 334, 128 and 64 alike); clearing hidden weights or taking 2^-126 off
+// again costs 3 to 8 % at 128.
 template <typename T, int HD>
-constexpr int kChunkExpFma = Pair16<T>::kBf16 ? 0 : HD <= 32 ? 3 : 2;
+constexpr int kChunkExpFma = !Pair16<T>::kBf16 && HD >= 128 ? 2 : 0;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(PagedChunkLayout<HD>::THREADS, 1)
