@@ -232,3 +232,52 @@ def test_hidden_values_weigh_nothing(tt_lib, dtype, hd, heads):
     assert torch.equal(late[:72], none[:72])  # positions 28 .. 99
     late, none = call(big, 0, 60, 30), call(0.0, 0, 60, 30)
     assert torch.equal(late[62:], none[62:])  # positions 90 .. 227 see 61 and later
+
+
+# ------------------------------------------------------------------------------------- strides of single entries
+def odd(t, **strides):
+    """t with other strides in dimensions of size one (named d0, d1, ...): the same elements."""
+    st = list(t.stride())
+    for name, s in strides.items():
+        assert t.shape[int(name[1:])] == 1
+        st[int(name[1:])] = s
+    return t.as_strided(t.shape, st)
+
+
+@gpu
+@pytest.mark.parametrize("total,window", [(40, 0), (9000, 0), (9000, 33)])
+def test_strides_of_single_entries_do_not_matter(tt_lib, total, window):
+    """One token, one head, one page, one slot, one layer: the stride of that dimension addresses nothing."""
+    book = Book(4, [total], 1, 64, 32, torch.float16, spare=0)
+    k, v, lens, cu = book.pages_k, book.pages_v, book.lens, ints([0, 1])
+    q = torch.randn(1, 4, 64, device=DEV).half()
+    want = ops.paged_attention(q, k, v, book.tables, lens, cu, window=window)
+    for args in ((odd(q, d0=7), k, v, book.tables), (q, odd(k, d1=5), odd(v, d1=3), book.tables),
+                 (q, k, v, odd(book.tables, d0=1))):
+        assert torch.equal(ops.paged_attention(*args, lens, cu, window=window), want)
+    wide, short = ints([[int(book.tables[0, 0]), 5, 7]]), ints([9])  # (a page whose rows all hold values)
+    args = (q, k, v, wide[:, ::2][:, :1], short, cu), (q, k, v, wide[:, :1], short, cu)
+    assert torch.equal(ops.paged_attention(*args[0]), ops.paged_attention(*args[1]))
+    one = torch.randn(33, 1, 64, device=DEV).half()
+    want = ops.paged_attention(one, k, v, book.tables, lens, ints([0, 33]))
+    assert torch.equal(ops.paged_attention(odd(one, d1=9), k, v, book.tables, lens, ints([0, 33])), want)
+
+
+@gpu
+def test_append_and_compact_ignore_strides_of_single_entries(tt_lib):
+    tables, lens, cu = ints([[0, -1]]), ints([7]), ints([0, 1])
+    new = torch.randn(1, 2, 32, device=DEV).half()
+    k = torch.zeros(1, 2, 16, 32, dtype=torch.float16, device=DEV)
+    want = k.clone()
+    want[0, :, 6] = new[0]
+    got = [torch.zeros_like(k) for _ in range(2)]
+    ops.cache_append(odd(new, d0=3), odd(new, d0=5), odd(got[0], d0=11), odd(got[1], d0=1), tables, lens, cu)
+    assert torch.equal(got[0], want) and torch.equal(got[1], want)
+    turned = new.transpose(1, 2).contiguous().transpose(1, 2)  # dense in nothing but the token
+    got = [torch.zeros_like(k) for _ in range(2)]
+    ops.cache_append(odd(turned, d0=3), odd(turned, d0=64), *got, tables, lens, cu)
+    assert torch.equal(got[0], want) and torch.equal(got[1], want)
+    k1 = torch.randn(1, 3, 1, 16, 32, device=DEV).half()
+    k2, refs, table = k1.clone(), ints([0, 0, 1]), ints([[2]])
+    ops.cache_compact(odd(k1, d0=13, d2=1), odd(k2, d0=3, d2=7), table, ints([16]), refs)
+    assert table.tolist() == [[0]] and torch.equal(k1[:, 0], k1[:, 2]) and torch.equal(k1, k2)

@@ -26,13 +26,15 @@ int guarded(F f) {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Checks the fields of a cache that every call uses, plus what `values` (K and
-// V) and `counts` (refs) ask for, and fills the kernels' parameters.
+// V) and `counts` (refs) ask for, and fills the kernels' parameters.  The stride
+// of a dimension of one entry addresses nothing: any will do, here and below.
 int cache_params(const tt_kv_cache* c, bool values, bool counts, CacheParams* out) {
   if (!c || !c->tables || !c->lens || (counts && !c->refs) || (values && (!c->k || !c->v)))
     return fail(TT_ERR_ARG, "null cache field");
   if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128 && c->page != 256)
     return fail(TT_ERR_UNSUPPORTED, "page %d not in {16, 32, 64, 128, 256}", c->page);
-  if (c->n_slots <= 0 || c->table_width <= 0 || c->n_pages <= 0 || c->table_stride < c->table_width)
+  if (c->n_slots <= 0 || c->table_width <= 0 || c->n_pages <= 0 ||
+      (c->n_slots > 1 && c->table_stride < c->table_width))
     return fail(TT_ERR_SHAPE, "invalid slots, table width, table stride or pages (%d, %d, %lld, %d)", c->n_slots,
                 c->table_width, static_cast<long long>(c->table_stride), c->n_pages);
   if (static_cast<long long>(c->table_width) * c->page >= 1LL << 30)
@@ -53,17 +55,19 @@ int cache_params(const tt_kv_cache* c, bool values, bool counts, CacheParams* ou
     return fail(TT_ERR_SHAPE, "invalid layers or kv_heads (%d, %d)", c->layers, c->kv_heads);
   const long long page_elems = static_cast<long long>(c->kv_heads) * c->page * c->head_dim;
   if (page_elems > 0x3fffffffLL) return fail(TT_ERR_SHAPE, "a page of %lld values is too large", page_elems);
-  if (!aligned16(c->k) || !aligned16(c->v) ||
-      (c->k_page_stride | c->v_page_stride | c->k_layer_stride | c->v_layer_stride) % 8 != 0)
+  const long long k_page = c->n_pages > 1 ? c->k_page_stride : page_elems;
+  const long long v_page = c->n_pages > 1 ? c->v_page_stride : page_elems;
+  const long long k_layer = c->layers > 1 ? c->k_layer_stride : 0, v_layer = c->layers > 1 ? c->v_layer_stride : 0;
+  if (!aligned16(c->k) || !aligned16(c->v) || (k_page | v_page | k_layer | v_layer) % 8 != 0)
     return fail(TT_ERR_ALIGN, "pools must be 16-byte aligned and their strides multiples of 8 elements");
-  if (c->k_page_stride < page_elems || c->v_page_stride < page_elems)
+  if (k_page < page_elems || v_page < page_elems)
     return fail(TT_ERR_SHAPE, "page strides are smaller than a page (%lld values)", page_elems);
   out->k = static_cast<uint8_t*>(c->k);
   out->v = static_cast<uint8_t*>(c->v);
-  out->k_layer = c->k_layer_stride * 2;
-  out->v_layer = c->v_layer_stride * 2;
-  out->k_stride = c->k_page_stride * 2;
-  out->v_stride = c->v_page_stride * 2;
+  out->k_layer = k_layer * 2;
+  out->v_layer = v_layer * 2;
+  out->k_stride = k_page * 2;
+  out->v_stride = v_page * 2;
   out->layers = c->layers;
   out->kv_heads = c->kv_heads;
   out->row_bytes = c->head_dim * 2;
@@ -257,11 +261,12 @@ int tt_cache_append(const tt_kv_cache* cache, const void* k, const int64_t* k_st
     const int64_t* st[2] = {k_strides, v_strides};
     for (int i = 0; i < 2; ++i) {
       const char* name = i ? "v" : "k";
-      src[i] = {static_cast<const uint16_t*>(ptr[i]), st[i][0], st[i][1], st[i][2]};
+      src[i] = {static_cast<const uint16_t*>(ptr[i]), st[i][0], c.kv_heads > 1 ? st[i][1] : 0, st[i][2]};
+      if (n_tokens == 1) src[i].token = st[i][2] == 1 ? 0 : 1;
       if (st[i][2] == 1) {
-        if (!aligned16(ptr[i]) || st[i][0] % 8 != 0 || st[i][1] % 8 != 0)
+        if (!aligned16(ptr[i]) || src[i].token % 8 != 0 || src[i].head % 8 != 0)
           return fail(TT_ERR_ALIGN, "%s rows must be 16-byte aligned", name);
-      } else if (st[i][0] != 1) {
+      } else if (src[i].token != 1) {
         return fail(TT_ERR_ARG, "%s must be dense in its features or in its tokens", name);
       }
     }
@@ -390,6 +395,8 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
                                         static_cast<long long>(c.table_width) << c.page_shift);
     if (!items && (!workspace || workspace_bytes < need))
       return fail(TT_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
+    if (n_tokens == 1) q_token_stride = static_cast<int64_t>(heads) * cache->head_dim;
+    if (heads == 1) q_head_stride = cache->head_dim;
     if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || q_token_stride % 8 != 0 || q_head_stride % 8 != 0)
       return fail(TT_ERR_ALIGN, "q, out and workspace must be 16-byte aligned, q's strides multiples of 8");
     if (n_tokens == 0) return TT_OK;
@@ -400,8 +407,8 @@ int tt_paged_attention(const tt_kv_cache* cache, const void* q, int64_t q_token_
     p.q_head = q_head_stride;
     p.k_pages = cache->k;
     p.v_pages = cache->v;
-    p.k_stride = cache->k_page_stride;
-    p.v_stride = cache->v_page_stride;
+    p.k_stride = c.k_stride / 2;
+    p.v_stride = c.v_stride / 2;
     p.tables = c.tables;
     p.table_stride = c.table_stride;
     p.lens = c.lens;

@@ -198,7 +198,7 @@ def _index(t: Optional[torch.Tensor], name: str, device: int, dims: int = 1) -> 
     if t is None:
         return 0
     if t.dtype is not torch.int32 or t.get_device() != device or t.dim() != dims or (
-            t.stride(1) != 1 if dims == 2 else not t.is_contiguous()):
+            t.stride(1) != 1 < t.shape[1] if dims == 2 else not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on cuda:{device}")
     return t.data_ptr()
 
@@ -233,7 +233,7 @@ def _cache(k: Optional[torch.Tensor], v: Optional[torch.Tensor], tables: torch.T
         shape, ks, vs = shape[1:], ks[1:], vs[1:]
     pages, kv_heads, page, head_dim = shape
     dense = (page * head_dim, head_dim, 1)
-    if ks[1:] != dense or vs[1:] != dense:
+    if (ks[1:] != dense or vs[1:] != dense) and not (kv_heads == 1 and ks[2:] == vs[2:] == dense[1:]):
         raise ValueError("each page of k and v must be contiguous")
     if refs is not None and refs.shape[0] != pages:
         raise ValueError(f"refs must have one entry for each of the {pages} pages")
