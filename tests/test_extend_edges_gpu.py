@@ -75,3 +75,29 @@ def test_tokens_at_any_address(tt_lib):
     assert torch.equal(got, want)
     with pytest.raises(_lib.TTError, match="aligned"):
         ops.layernorm_rows(x, model.layers[0].norm1.weight, model.layers[0].norm1.bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,heads,ffn", [(128, 4, 128), (512, 8, 2048)])
+def test_tokens_from_a_captured_graph(tt_lib, d, heads, ffn):
+    """extend(check=False) captured once gives, replayed token by token, the rows of the same calls made one by one."""
+    cfg, sd, model = build(d, heads, ffn, 2, batch=2, seq=64)
+    prompt, steps = torch.randn(2, 37, d, device=DEV), torch.randn(12, 2, 1, d, device=DEV)
+    one, two = (PagedKVCache.for_model(model, slots=2, max_len=64, page=16) for _ in range(2))
+    with torch.inference_mode():
+        for cache in (one, two):
+            model.extend(prompt, cache)
+        want = [model.extend(x, one) for x in steps]
+        x = steps[0].clone()
+        warm = PagedKVCache.for_model(model, slots=2, max_len=64, page=16)
+        model.extend(x, warm, check=False)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = model.extend(x, two, check=False)
+        for step, row in zip(steps, want):
+            x.copy_(step)
+            graph.replay()
+            assert torch.equal(out, row)
+        two.check()
+    assert two.lens.tolist() == one.lens.tolist() == [49, 49]

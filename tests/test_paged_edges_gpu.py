@@ -281,3 +281,60 @@ def test_append_and_compact_ignore_strides_of_single_entries(tt_lib):
     k2, refs, table = k1.clone(), ints([0, 0, 1]), ints([[2]])
     ops.cache_compact(odd(k1, d0=13, d2=1), odd(k2, d0=3, d2=7), table, ints([16]), refs)
     assert table.tolist() == [[0]] and torch.equal(k1[:, 0], k1[:, 2]) and torch.equal(k1, k2)
+
+
+# ------------------------------------------------------------------------------- groupings and routes less travelled
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [16, 64, 128, 256])
+@pytest.mark.parametrize("group", [9, 15, 16, 17, 31, 64, 100, 127, 128])
+def test_attention_large_groups(tt_lib, dtype, hd, group):
+    """9 to 128 query heads to a KV head; from 17 on single tokens take the chunk kernel too."""
+    news, past = [1, 1, 5, 40, 0, 2], [0, 700, 64, 100, 9, 2000]
+    book = Book(hd + group, [n + p for n, p in zip(news, past)], 2, hd, 32, dtype)
+    check_attention(book, news, 2 * group, dtype)
+    check_attention(book, news, 2 * group, dtype, window=33, sinks=2, layout="heads")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (3000, 65)])
+def test_attention_short_rows_over_wide_tables(tt_lib, dtype, hd, window, sinks):
+    """The rows kernel and its join at every head_dim: ragged tokens, some over caches that are cut."""
+    news, past, kv_heads, heads = call_of("rows", hd)
+    book = Book(hd + 7, [n + p for n, p in zip(news, past)], kv_heads, hd, 64, dtype)
+    check_attention(book, news, heads, dtype, window=window, sinks=sinks)
+
+
+@gpu
+@pytest.mark.parametrize("route", ["rows", "few", "chunk"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_head_dim_8_on_every_kernel(tt_lib, route, dtype):
+    news, past, kv_heads, heads = call_of(route, 16)
+    book = Book(12, [n + p for n, p in zip(news, past)], kv_heads, 16, 32, dtype)
+    check_attention(book, news, heads, dtype, hd_out=8)
+
+
+@gpu
+@pytest.mark.parametrize("hd,dtype,kv_heads,group", [(16, torch.bfloat16, 4, 1), (32, torch.float16, 3, 2),
+                                                     (64, torch.bfloat16, 2, 5), (128, torch.bfloat16, 4, 1),
+                                                     (256, torch.float16, 2, 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 4)])
+def test_attention_chunks_and_tokens_in_two_launches(tt_lib, hd, dtype, kv_heads, group, window, sinks):
+    """More than two (sequence, KV head) pairs per SM: longer chunks and short rows go by their own kernels."""
+    n = 320 // kv_heads + 60
+    news = [40 if i % 16 == 0 else (i % 3) for i in range(n)]
+    past = [(37 * i) % 90 for i in range(n)]
+    past[3] = LONG[hd]
+    book = Book(hd + kv_heads, [a + b for a, b in zip(news, past)], kv_heads, hd, 32, dtype)
+    check_attention(book, news, kv_heads * group, dtype, window=window, sinks=sinks)
+
+
+@gpu
+@pytest.mark.parametrize("hd,group,page", [(128, 4, 64), (64, 1, 16), (32, 1, 128), (256, 2, 32), (16, 5, 16)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (129, 67), (1000, 4), (5000, 9)])
+def test_attention_window_bf16(tt_lib, hd, group, page, window, sinks):
+    news, past = [1, 1, 7, 40, 300, 1, 129], [0, 3000, 100, 1500, 64, 130, 1000]
+    book = Book(window + hd, [n + p for n, p in zip(news, past)], 1, hd, page, torch.bfloat16)
+    check_attention(book, news, group, torch.bfloat16, window=window, sinks=sinks)
