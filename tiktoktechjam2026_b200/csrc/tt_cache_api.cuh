@@ -197,10 +197,14 @@ int launch_paged(const PagedParams& p, bool items, int max_rows, int sm_count, c
   if (items) return launch_paged_item<T, HD>(p, stream);
   const long long pairs = static_cast<long long>(p.batch) * p.kv_heads;
   // With a handful of (sequence, KV head) pairs a piece for every warp would
-  // divide an item into a hundred parts; the chunk kernel has a piece per SM.
-  // One token over 8000 keys, 4 heads to each KV head of 128, in us, chunk
-  // kernel and this: 8 pairs 34 and 52, 16 pairs 38 and 44, 32 pairs 48 and 46.
-  constexpr int kFewPairs = 16;
+  // divide an item into a hundred parts, whose join grows with head_dim; the
+  // chunk kernel has a piece per SM.  Single tokens over 8000 keys, in us on the
+  // GPU, chunk kernel and this, with 8, 16 and 32 pairs:
+  //   4 heads to a KV head of 256: 33 44, 41 48, 60 72; of 128: 24 37, 27 32, 37 36;
+  //   of 64: 19 21, 23 22, 32 24; of 32: 17 13, 22 16, 31 19;
+  //   one head to it, 256: 27 31, 37 41, 58 67; 128: 21 23, 26 25, 37 33;
+  //   64: 18 17, 23 19, 32 23; 32: 17 13, 22 16, 31 19.
+  constexpr int kFewPairs = HD == 256 ? 32 : HD == 128 ? 16 : 0;
   if (max_rows <= kRowsMax && pairs > kFewPairs)
     return launch_paged_rows<T, HD>(p, 0, 0x7fffffff, sm_count, stream);
   // With few (sequence, KV head) pairs the chunk kernel takes short sequences
