@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kCacheThreads)
 // Carries the fork out: block (i, y) copies its share of the used rows of pair
 // i's partial page (layer and K or V by y); y = 0 also writes the child's
 // table row and counts the shared pages.  112 children over 4 layers of 8 heads
-// of 64 (51 MB): 14 us, 3.6 TB/s in runs of at most 4 KB (the plan before it 7).
+// of 64 (51 MB): 14 us, 3.6 TB/s in runs of at most 8 KB (the plan before it 7).
 __global__ void __launch_bounds__(256)
     cache_fork_kernel(const CacheParams c, const int* parents, const int* children, const int* scratch) {
   if (!scratch[0]) return;

@@ -137,7 +137,9 @@ int launch_paged_rows(PagedParams p, int row_lo, int row_hi, int sm_count, cudaS
 // cache in sight than a block streams in some 15 us.  In us, this against cut
 // pieces, 8 KV heads of 128: one sequence of 500 keys 13 and 20, of 8000 98 and
 // 52; 64 of 1000 54 and 62, 64 of 100 to 8000 217 and 193 (the last blocks run
-// alone).
+// alone).  Lengths are on the device, so without a window it is the table's
+// width that counts: the same short sequences in wider tables (at head_dim 64,
+// of more than 2560 tokens) take the cut pieces.
 constexpr long long kItemBytes = 640 * 1024;
 bool paged_item_route(int stored_hd, long long max_rows, int window, int sinks, long long room) {
   const long long reach = static_cast<long long>(window) + sinks + kRowsMax;  // keys that a window leaves an item

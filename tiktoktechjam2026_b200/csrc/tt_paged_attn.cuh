@@ -487,6 +487,13 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const PagedParams p
 //   S = Q K^T (mma.sync m16n8k16, FP32), online softmax on the fragments,
 //   O += P V with P rounded to the cache's type (the A operand's layout is the
 //   accumulator's, so P never leaves registers).
+// That rounding is the one besides the output's: mma.sync takes no wider A with
+// a 16-bit V, and P in two terms would double the P V instructions.  l sums
+// the unrounded P.  Against 64 bits it brings 2.0e-4 to 2.3-2.7e-4 in FP16 and
+// 1.7e-3 to 2.1-2.3e-3 in BF16 (relative norm; the output's rounding alone is the
+// first figure).
+// At head_dim 256 O and the queries leave the rows kernel short of registers: it
+// stores 136 bytes a thread outside them and loads 68.
 // Values of keys past the sequence's end are zero-filled by the copy: stale
 // rows of a page never reach the sum.
 // ---------------------------------------------------------------------------
@@ -568,101 +575,101 @@ struct PagedRows {
   __device__ __forceinline__ void start(const PagedParams& p, const PagedSeq& seq, const PagedItem<TK>& it, int kvh) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = min(lane / 4 + 8 * h, it.rows - 1) + it.r0;
-            const int tok = r / p.group, head = kvh * p.group + r % p.group;
-            pos[h] = seq.L - seq.T + tok;
-            const T* src = static_cast<const T*>(p.q) + (seq.q0 + tok) * p.q_token + head * p.q_head + lane % 4 * 2;
+    for (int h = 0; h < 2; ++h) {
+      const int r = min(lane / 4 + 8 * h, it.rows - 1) + it.r0;
+      const int tok = r / p.group, head = kvh * p.group + r % p.group;
+      pos[h] = seq.L - seq.T + tok;
+      const T* src = static_cast<const T*>(p.q) + (seq.q0 + tok) * p.q_token + head * p.q_head + lane % 4 * 2;
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-              qf[kk][h] = *reinterpret_cast<const uint32_t*>(src + kk * 16);
-              qf[kk][2 + h] = *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8);
-            }
-            m[h] = -INFINITY;
-            l[h] = 0.f;
-          }
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        qf[kk][h] = *reinterpret_cast<const uint32_t*>(src + kk * 16);
+        qf[kk][2 + h] = *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8);
+      }
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+    }
 #pragma unroll
-          for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
   }
 
   __device__ __forceinline__ void tile(const PagedParams& p, uint32_t sk, int k0, bool whole) {
     const int lane = threadIdx.x & 31;
     const uint32_t sv = sk + L::TILE;
-        float s[TK / 8][4];
+    float s[TK / 8][4];
 #pragma unroll
-        for (int n = 0; n < TK / 8; n += 2) {
-          float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < TK / 8; n += 2) {
+      float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            uint32_t b[4];  // keys 8n .. 8n+7 at features 0-7, 8-15, then keys 8n+8 .. 8n+15
-            ldmatrix_x4(sk + paged_rows_at<HD>(8 * n + (lane & 7) + (lane & 16 ? 8 : 0), 2 * kk + ((lane >> 3) & 1)), b);
-            PT::mma(s0, qf[kk], b[0], b[1]);
-            PT::mma(s1, qf[kk], b[2], b[3]);
-          }
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        uint32_t b[4];  // keys 8n .. 8n+7 at features 0-7, 8-15, then keys 8n+8 .. 8n+15
+        ldmatrix_x4(sk + paged_rows_at<HD>(8 * n + (lane & 7) + (lane & 16 ? 8 : 0), 2 * kk + ((lane >> 3) & 1)), b);
+        PT::mma(s0, qf[kk], b[0], b[1]);
+        PT::mma(s1, qf[kk], b[2], b[3]);
+      }
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            s[n][x] = s0[x] * p.scale_log2;
-            s[n + 1][x] = s1[x] * p.scale_log2;
-          }
+      for (int x = 0; x < 4; ++x) {
+        s[n][x] = s0[x] * p.scale_log2;
+        s[n + 1][x] = s1[x] * p.scale_log2;
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < TK / 8; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int key = k0 + 8 * n + lane % 4 * 2 + (x & 1), t = pos[x >> 1];
+          if (key > t || (p.window > 0 && t - key >= p.window && key >= p.sinks)) s[n][x] = -INFINITY;
         }
-        if (!whole) {
+    }
+    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int n = 0; n < TK / 8; ++n)
+    for (int n = 0; n < TK / 8; ++n) {
+      top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
+      top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]));
+    }
+    float base[2];
+    bool moved = false;
+    float corr[2];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int key = k0 + 8 * n + lane % 4 * 2 + (x & 1), t = pos[x >> 1];
-              if (key > t || (p.window > 0 && t - key >= p.window && key >= p.sinks)) s[n][x] = -INFINITY;
-            }
-        }
-        float top[2] = {-INFINITY, -INFINITY};
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
+      const float next = fmaxf(m[h], top[h]);
+      base[h] = next == -INFINITY ? 0.f : next;  // a row that has seen no key: every 2^(s - 0) below is 0
+      corr[h] = ex2_approx(m[h] - base[h]);
+      moved |= next > m[h];
+      m[h] = next;
+      l[h] *= corr[h];
+    }
+    if (__any_sync(~0u, moved)) {
 #pragma unroll
-        for (int n = 0; n < TK / 8; ++n) {
-          top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
-          top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]));
-        }
-        float base[2];
-        bool moved = false;
-        float corr[2];
+      for (int d = 0; d < HD / 8; ++d) {
+        o[d][0] *= corr[0];
+        o[d][1] *= corr[0];
+        o[d][2] *= corr[1];
+        o[d][3] *= corr[1];
+      }
+    }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
-          top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
-          const float next = fmaxf(m[h], top[h]);
-          base[h] = next == -INFINITY ? 0.f : next;  // a row that has seen no key: every 2^(s - 0) below is 0
-          corr[h] = ex2_approx(m[h] - base[h]);
-          moved |= next > m[h];
-          m[h] = next;
-          l[h] *= corr[h];
-        }
-        if (__any_sync(~0u, moved)) {
+    for (int n = 0; n < TK / 8; n += 2) {
+      uint32_t pf[4];
 #pragma unroll
-          for (int d = 0; d < HD / 8; ++d) {
-            o[d][0] *= corr[0];
-            o[d][1] *= corr[0];
-            o[d][2] *= corr[1];
-            o[d][3] *= corr[1];
-          }
-        }
+      for (int g = 0; g < 2; ++g) {
+        const float e0 = ex2_approx(s[n + g][0] - base[0]), e1 = ex2_approx(s[n + g][1] - base[0]);
+        const float e2 = ex2_approx(s[n + g][2] - base[1]), e3 = ex2_approx(s[n + g][3] - base[1]);
+        l[0] += e0 + e1;
+        l[1] += e2 + e3;
+        pf[2 * g] = PT::pack(e0, e1);
+        pf[2 * g + 1] = PT::pack(e2, e3);
+      }
 #pragma unroll
-        for (int n = 0; n < TK / 8; n += 2) {
-          uint32_t pf[4];
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float e0 = ex2_approx(s[n + g][0] - base[0]), e1 = ex2_approx(s[n + g][1] - base[0]);
-            const float e2 = ex2_approx(s[n + g][2] - base[1]), e3 = ex2_approx(s[n + g][3] - base[1]);
-            l[0] += e0 + e1;
-            l[1] += e2 + e3;
-            pf[2 * g] = PT::pack(e0, e1);
-            pf[2 * g + 1] = PT::pack(e2, e3);
-          }
-#pragma unroll
-          for (int d = 0; d < HD / 8; d += 2) {
-            uint32_t b[4];  // keys 8n .. 8n+15 (two halves) at features 8d .. 8d+7, then the next eight
-            ldmatrix_x4_trans(sv + paged_rows_at<HD>(8 * n + (lane & 15), d + (lane >> 4)), b);
-            PT::mma(o[d], pf, b[0], b[1]);
-            PT::mma(o[d + 1], pf, b[2], b[3]);
-          }
-        }
+      for (int d = 0; d < HD / 8; d += 2) {
+        uint32_t b[4];  // keys 8n .. 8n+15 (two halves) at features 8d .. 8d+7, then the next eight
+        ldmatrix_x4_trans(sv + paged_rows_at<HD>(8 * n + (lane & 15), d + (lane >> 4)), b);
+        PT::mma(o[d], pf, b[0], b[1]);
+        PT::mma(o[d + 1], pf, b[2], b[3]);
+      }
+    }
   }
 
   // Makes l the sums of whole rows.
@@ -800,7 +807,7 @@ __global__ void __launch_bounds__(32 * kItemWarps) paged_item_kernel(const Paged
   constexpr int SLOT = static_cast<int>(paged_slot_floats<16, HD>());
   static_assert(kItemWarps * SLOT * 4 + 128 <= kItemSmem<HD>, "the parts take the ring's place");
   extern __shared__ uint8_t smem_raw[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
   const uint32_t ring = smem_u32(smem) + warp * NST * L::STAGE;
   float* parts = reinterpret_cast<float*>(smem);

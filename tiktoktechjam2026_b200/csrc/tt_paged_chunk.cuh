@@ -18,17 +18,22 @@
 // sequence's end in its last page may hold anything (0 * NaN would reach the
 // sum): the score issuer of half 0 zeroes them in shared memory.
 //
+// P is rounded to the cache's type, which the tensor core takes beside a 16-bit V;
+// m, l (of the unrounded P) and O are FP32.  Against 64 bits that brings 2.0e-4
+// to 2.6-2.7e-4 in FP16 and 1.7e-3 to 2.4e-3 in BF16 (relative norm; the output's
+// rounding alone is the first figure).
+//
 // What bounds it: a tile of 64 keys x 256 rows takes 1700-1850 cycles.  At
 // head_dim 128 the tensor core needs 1280 of them (Q K^T with N = 64 runs at 48
 // cycles per MMA, the rate of its operand reads from shared memory; P V at 64)
-// and is active 59 % of the time at the 1.54 GHz that the power limit leaves
-// (2048 new tokens over 30k keys, 16 heads over 4: 1.03 PFLOP/s).  Below that
+// and is active 55 % of the time at the 1.62 GHz that the power limit leaves
+// (2048 new tokens over 30k keys, 16 heads over 4, BF16: 1.03 PFLOP/s).  Below that
 // the softmax warps bound it, two per scheduler and each a chain of TMEM read,
 // maximum, exponentials, TMEM write.  Measured and left out: key tiles of 128
 // with P over S (one S buffer: the halves fall into step and wait for the
 // tensor core together, 4946 cycles per 128 keys) or beside it (582 us where
 // this takes 508); one issuing warp per half (550); more code than the
-// instruction cache holds (141 KB of it: 104 us for 32 prompts, 86 now).
+// instruction cache holds (141 KB of it: 104 us for 32 prompts, 85 now).
 #pragma once
 
 #include "tt_attention.cuh"  // max3
