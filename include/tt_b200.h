@@ -259,7 +259,8 @@ int tt_cache_copy_pages(const tt_kv_cache* cache, const int* src, const int* dst
  * out[row, h*hd:(h+1)*hd] = softmax(scale q k^T) v over the visible keys, zero
  * for a row that sees none and for a row of no sequence; FP32 statistics and
  * accumulation, out in the cache's type.  scale: any finite value (times log2 e
- * too), negative and zero ones included.  q: [n_tokens, heads, stored
+ * too), negative and zero ones included; scaled scores of at most 2^26 (from
+ * there on FP32 keeps less than whole units of them, and a row may be NaN).  q: [n_tokens, heads, stored
  * head_dim], element strides token and head, multiples of 8; query head h
  * reads KV head h / (heads / kv_heads), heads / kv_heads <= 128; fewer than
  * 2^30 query rows (tokens times heads / kv_heads).  head_dim: 8

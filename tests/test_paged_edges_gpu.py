@@ -3,16 +3,18 @@
 Attention is held to the 64-bit formula and tolerance of ``test_paged_gpu``; everything else is compared exactly.
 """
 
+import math
+
 import pytest
 import torch
 
-from test_paged_gpu import DEV, Book, check_attention, ints
+from test_paged_gpu import DEV, UNIT, Book, attention_64, check_attention, ints
 from tiktoktechjam2026_b200 import PagedKVCache, _lib, ops
 
 gpu = pytest.mark.gpu
 
 # Calls for each kernel of the attention: (new tokens, tokens before them, KV heads, query heads).  "item": short rows
-# over short tables; "rows": short rows, tables past 640 KB of cache, more than 16 (sequence, KV head) pairs; "chunk":
+# over short tables; "rows": short rows, tables past 640 KB of cache, more than 32 (sequence, KV head) pairs; "chunk":
 # more than 16 rows; "few": short rows over a long cache, at most 16 pairs.
 LONG = {16: 11000, 32: 6000, 64: 3000, 128: 1500, 256: 800}
 
@@ -21,7 +23,7 @@ def call_of(route, hd):
     if route == "item":
         return [1, 2, 3, 1], [0, 15, 297, 63], 2, 4
     if route == "rows":
-        return [1, 2, 1, 4, 1, 1, 3, 1, 1], [LONG[hd], 5, 64, 700, 0, 129, LONG[hd] // 2, 1, 300], 2, 4
+        return [1, 2, 1, 4, 1, 1, 3, 1, 1], [LONG[hd], 5, 64, 700, 0, 129, LONG[hd] // 2, 1, 300], 4, 8
     if route == "few":
         return [1, 3], [LONG[hd], 70], 2, 4
     return [1, 130, 40, 300], [300, 64, 500, 0], 2, 4
@@ -338,3 +340,58 @@ def test_attention_window_bf16(tt_lib, hd, group, page, window, sinks):
     news, past = [1, 1, 7, 40, 300, 1, 129], [0, 3000, 100, 1500, 64, 130, 1000]
     book = Book(window + hd, [n + p for n, p in zip(news, past)], 1, hd, page, torch.bfloat16)
     check_attention(book, news, group, torch.bfloat16, window=window, sinks=sinks)
+
+
+# ------------------------------------------------------------------------------------------ huge scores
+def _equal_keys(route, hd, dtype, size, sign, top):
+    """Rows whose scores are sign * hd ** 0.5 * size ** 2, or `top` times that for every third key -> (own, o, a)."""
+    news, past, kv_heads, heads = call_of(route, hd)
+    book = Book(hd + 3, [n + p for n, p in zip(news, past)], kv_heads, hd, 64, dtype)
+    book.pages_k[~torch.isnan(book.pages_k)] = size
+    q = torch.full((sum(news), heads, hd), sign * size, device=DEV).to(dtype)
+    cu = [0]
+    for b, slot in enumerate(book.slot_of):
+        row = book.tables[slot].tolist()
+        book.k[b][:] = float(torch.tensor(size).to(dtype))
+        book.k[b][::3] *= top
+        for u in range(0, book.k[b].shape[0], 3):
+            book.pages_k[row[u // 64], :, u % 64] *= top
+        cu.append(cu[-1] + news[b])
+    got = ops.paged_attention(q, book.pages_k, book.pages_v, book.tables, book.lens, ints(cu), slots=book.slots,
+                              max_q_len=max(news))
+    got = got.cpu().double().view(-1, heads, hd)
+    for b in range(len(news)):
+        o, a = attention_64(q[cu[b]:cu[b + 1]].cpu().double(), book.k[b], book.v[b], hd**-0.5, 0, 0)
+        yield got[cu[b]:cu[b + 1]], o, a, book.k[b].shape[0] * 2.0**-25 * float(book.v[b].abs().max()) + 2.0**-24
+
+
+@gpu
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 60000.0), (torch.bfloat16, 60000.0), (torch.bfloat16, 2.0**50)])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("route", ["item", "rows"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attention_short_rows_huge_scores(tt_lib, dtype, size, hd, route, sign):
+    """Queries and keys near the type's largest: equal scores give the mean, a larger one takes its row."""
+    u = UNIT[dtype]
+    for top in (1.0, 0.5):
+        for got, o, a, small in _equal_keys(route, hd, dtype, size, sign, top):
+            assert torch.all((got - o).abs() <= 2 * u * o.abs() + 2 * u * a + 2e-4 * a + small)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("route", ["few", "chunk"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("bits", [10, 20, 26])
+def test_attention_large_scores(tt_lib, dtype, hd, route, sign, bits):
+    """Scaled scores of 2^9 to 2^26 (log2 e included): a score s counts to s 2^-23, so that two weights of a row differ
+    by a factor of at most 2^(s 2^-22) from the formula's."""
+    size = float(2.0 ** ((bits - 0.5 * math.log2(hd) - math.log2(math.log2(math.e))) / 2) * 0.99)
+    size = float(torch.tensor(size).to(dtype))
+    s, u = hd**0.5 * size * size * math.log2(math.e), UNIT[dtype]
+    assert 2.0 ** (bits - 1) <= s <= 2.0**bits
+    for got, o, a, small in _equal_keys(route, hd, dtype, size, sign, 1.0):
+        vmax = 8.0  # a row lies within its values, whatever their weights
+        tol = (2.0 ** min(s * 2.0**-22, 8.0) - 1) * a + 2 * u * o.abs() + 2 * u * a + 2e-4 * a + small
+        assert torch.all((got - o).abs() <= tol) and torch.all(got.abs() <= vmax)

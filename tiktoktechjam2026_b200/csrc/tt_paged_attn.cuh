@@ -608,8 +608,10 @@ struct PagedRows {
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        s[n][x] = s0[x] * p.scale_log2;
-        s[n + 1][x] = s1[x] * p.scale_log2;
+        // (Never contracted into the subtraction of m below: m is such a product, rounded, and a huge score's rounding
+        // would become an exponent.)
+        s[n][x] = __fmul_rn(s0[x], p.scale_log2);
+        s[n + 1][x] = __fmul_rn(s1[x], p.scale_log2);
       }
     }
     if (!whole) {

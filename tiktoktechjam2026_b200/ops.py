@@ -382,7 +382,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     q [tokens, heads, hs] (dense features, any token and head strides of whole 16 bytes); heads a
     multiple of the pages' kv_heads.  The T new tokens of a sequence are its last T positions
-    (``lens`` counts them).  ``scale`` (hd ** -0.5 by default) is any finite number.  With ``window``
+    (``lens`` counts them).  ``scale`` (hd ** -0.5 by default) is any finite number; scaled
+    scores are at most 2^26 (FP32 keeps less than whole units of larger ones).  With ``window``
     a query sees the last ``window`` keys, itself included, and the first ``sinks`` ones.  A row that
     sees no key, or belongs to no sequence, is zero.
     ``head_dim`` 8 takes pages stored 16 wide; ``max_q_len``, if known, bounds every T.
