@@ -395,3 +395,11 @@ def test_attention_large_scores(tt_lib, dtype, hd, route, sign, bits):
         vmax = 8.0  # a row lies within its values, whatever their weights
         tol = (2.0 ** min(s * 2.0**-22, 8.0) - 1) * a + 2 * u * o.abs() + 2 * u * a + 2e-4 * a + small
         assert torch.all((got - o).abs() <= tol) and torch.all(got.abs() <= vmax)
+
+
+@gpu
+def test_attention_without_heads_is_refused(tt_lib):
+    book = Book(1, [20, 40], 2, 32, 16, torch.float16)
+    q = torch.randn(2, 4, 32, device=DEV).half()
+    with pytest.raises(ValueError, match="heads"):
+        ops.paged_attention(q[:, :0], book.pages_k, book.pages_v, book.tables, book.lens, ints([0, 1, 2]))

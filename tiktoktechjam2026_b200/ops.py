@@ -401,11 +401,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     dtype = q.dtype
     if dtype is not k_pages.dtype or q.get_device() != dev:
         raise ValueError("q must have the pages' dtype and device")
-    if heads % c.kv_heads:
+    if heads % c.kv_heads or not heads:
         raise ValueError(f"{heads} query heads are not a multiple of {c.kv_heads} KV heads")
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
-    window, sinks = _reach(window), _reach(sinks)
+    if window > 1 << 30 or sinks > 1 << 30:
+        window, sinks = _reach(window), _reach(sinks)
     hd = hs if head_dim is None else int(head_dim)
     cu, sl, batch = _batch(cu_q, slots, tables)
     if out is None:
