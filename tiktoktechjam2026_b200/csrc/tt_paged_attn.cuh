@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const PagedParams p
 //   accumulator's, so P never leaves registers).
 // That rounding is the one besides the output's: mma.sync takes no wider A with
 // a 16-bit V, and P in two terms would double the P V instructions.  l sums
-// the unrounded P.  Against 64 bits it brings 2.0e-4 to 2.3-2.7e-4 in FP16 and
+// the unrounded P.  Against 64 bits it brings 2.0-2.3e-4 to 2.3-2.8e-4 in FP16 and
 // 1.7e-3 to 2.1-2.3e-3 in BF16 (relative norm; the output's rounding alone is the
 // first figure).
 // At head_dim 256 O and the queries leave the rows kernel short of registers: it

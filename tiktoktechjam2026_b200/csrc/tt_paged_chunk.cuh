@@ -19,8 +19,8 @@
 // sum): the score issuer of half 0 zeroes them in shared memory.
 //
 // P is rounded to the cache's type, which the tensor core takes beside a 16-bit V;
-// m, l (of the unrounded P) and O are FP32.  Against 64 bits that brings 2.0e-4
-// to 2.6-2.7e-4 in FP16 and 1.7e-3 to 2.4e-3 in BF16 (relative norm; the output's
+// m, l (of the unrounded P) and O are FP32.  Against 64 bits that brings 1.7-2.0e-4
+// to 2.4-2.7e-4 in FP16 and 1.7e-3 to 2.4e-3 in BF16 (relative norm; the output's
 // rounding alone is the first figure).
 //
 // What bounds it: a tile of 64 keys x 256 rows takes 1700-1850 cycles.  At
